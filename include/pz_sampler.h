@@ -76,8 +76,8 @@ typedef struct {
 
 /* Creates a sampler on `device` for batches of up to max_batch rows of up to
  * max_vocab logits and histories of up to max_hist ids (max_hist <= 2048).
- * Allocates all its device memory but the workspaces of verification and of
- * long attention rows, which their first calls allocate.  The largest part is
+ * Allocates all its device memory but the workspaces of verification, of long
+ * attention rows and of tree attention, which their first calls allocate.  The largest part is
  * the scratch that sorts top-p rows with wide nuclei: 16 bytes per id (ids
  * rounded up to a power of two, at most 262144) for each row sorted at once,
  * which is min(max_batch, compute units) rows while that is at most a 64th of
@@ -347,6 +347,152 @@ PZ_API int pz_lm_head_bf16(pz_sampler *s, const uint16_t *d_w, int V, int n,
  * are written.  Asynchronous on the sampler's stream. */
 PZ_API int pz_lm_head_argmax_bf16(pz_sampler *s, const uint16_t *d_w, int V, int n,
                                   const float *d_x, int B, long ldx, int32_t *d_ids);
+
+/* Element types of the calls that take more than one. */
+#define PZ_F32  0
+#define PZ_BF16 1 /* bit patterns: the upper half of an fp32 */
+#define PZ_F16  2 /* IEEE binary16 */
+
+/* Logit rules: what changes logits between the LM head and the sampler.  All
+ * pointers are device memory, and NULL where the rule is not used.
+ *   history: id i seen c > 0 times among the row's first min(d_hist_len[r], H)
+ *     entries of d_hist [B, H] (d_hist_len NULL: all H; ids outside [0, V)
+ *     are ignored): x>0 ? x/rep : x*rep, then x -= (float)c*frequency +
+ *     presence, the penalties of pz_row_params, without a limit on H.
+ *     d_penalties [B, 3] gives each row its own {rep, presence, frequency}
+ *     in place of the three here.
+ *   biases: then x += d_bias[r, e] for every entry e of d_bias_ids
+ *     [B, n_bias] that names the id, in the list's order (entries outside
+ *     [0, V) are ignored: pad with -1).
+ *   mask: then x = -infinity where bit i % 32 of word i / 32 is 0 in the
+ *     row's mask: row d_mask_row[r] of d_mask [n_masks, ld_mask] (words), or
+ *     row r when d_mask_row is NULL (n_masks must then be B).  An index
+ *     outside [0, n_masks) leaves the row unmasked, so that constrained and
+ *     unconstrained rows share a call and states share a mask.
+ *   d_allowed [B]: receives how many ids the row's mask allows (V without
+ *     one).  A row that allows none is -infinity throughout and reads 0. */
+typedef struct {
+  float rep_penalty;       /* 1: off */
+  float presence_penalty;  /* 0: off */
+  float frequency_penalty; /* 0: off */
+  const float *d_penalties;
+  const int32_t *d_hist;
+  int H;
+  const int32_t *d_hist_len;
+  const int32_t *d_bias_ids;
+  const float *d_bias;
+  int n_bias;
+  const uint32_t *d_mask;
+  long ld_mask;
+  int n_masks;
+  const int32_t *d_mask_row;
+  int32_t *d_allowed;
+} pz_logit_rules;
+
+/* Applies the rules to B rows of V logits: d_out[r, i] from d_in[r, i], bit
+ * for bit as above in fp32.  d_out == d_in (with ld_out == ld_in) works in
+ * place, which writes only the ids that a rule names and those the mask rules
+ * out; otherwise the two must not overlap, and every d_out[r, 0 .. V) is
+ * written.  For the samplers' rows and for verification's (B * (K + 1) rows,
+ * each with its own history); no limit by the sampler's max_batch, max_vocab
+ * or max_hist.  Reads *rules during the call only.  Asynchronous on the
+ * sampler's stream; uses no workspace and can be captured into a HIP graph. */
+PZ_API int pz_rules_batch(pz_sampler *s, const float *d_in, long ld_in, float *d_out,
+                          long ld_out, int B, int V, const pz_logit_rules *rules);
+
+/* Rows to 8-bit integers with a scale each, symmetric: scale = max|x| / 127,
+ * q = x / scale rounded to the nearest integer (halves to even) and clamped to
+ * +-127, both quotients correctly rounded fp32.  d_x: device [rows, ldx] of
+ * x_type (PZ_F32, PZ_BF16, PZ_F16); d_q: device [rows, ldq] int8; d_scale:
+ * device [rows].  A row of zeros (or one whose scale underflows) gets scale 0
+ * and zeros; a row holding an infinity or NaN gets scale NaN and zeros, so
+ * that what is computed from it is NaN.  For activations (a row per token)
+ * and for weights (a row per output channel).  Asynchronous on the sampler's
+ * stream. */
+PZ_API int pz_quant_rows_i8(pz_sampler *s, const void *d_x, int x_type, long ldx, int rows,
+                            int n, int8_t *d_q, long ldq, float *d_scale);
+
+/* The LM head in 8-bit integers, for B quantised activation rows at once:
+ *   d_logits[b, i] = (fl32(sum_j d_w[i, j] * d_x[b, j]) * d_sw[i]) * d_sx[b]
+ * d_w: device [V, n] int8 with a scale per row (channel) in d_sw [V]; d_x:
+ * device [B, ldx] int8 with a scale per row (token) in d_sx [B].  The sum is
+ * exact (int32; n <= PZ_I8_MAX_N, PZ_ERANGE beyond), so every logit is the
+ * formula's to the bit, in any batch.  Half the bytes of pz_lm_head_bf16's
+ * weights.  B <= max_batch.  Rows of d_w and d_x that start 16-byte aligned
+ * (n and ldx multiples of 16) are the quick case.  Asynchronous on the
+ * sampler's stream. */
+#define PZ_I8_MAX_N 131071
+PZ_API int pz_lm_head_i8(pz_sampler *s, const int8_t *d_w, const float *d_sw, int V, int n,
+                         const int8_t *d_x, const float *d_sx, int B, long ldx,
+                         float *d_logits, long ld);
+
+/* The same product with greedy sampling fused into its epilogue, as
+ * pz_lm_head_argmax_bf16: d_ids[b] is the argmax of exactly the logits
+ * pz_lm_head_i8 writes (the first maximum; a NaN logit 0 gives 0).
+ * Asynchronous on the sampler's stream. */
+PZ_API int pz_lm_head_argmax_i8(pz_sampler *s, const int8_t *d_w, const float *d_sw, int V, int n,
+                                const int8_t *d_x, const float *d_sx, int B, long ldx,
+                                int32_t *d_ids);
+
+/* A paged cache of keys and values, caller-owned, on the device.  Position p
+ * of sequence b lies in slot d_blocks[b, p / block_size] * block_size +
+ * p % block_size (d_blocks: [B, max_blocks] page numbers); slot i's n_kv_heads
+ * x head_dim keys start at d_k + i * ld elements, its values at d_v + i * ld.
+ * d_len [B]: positions that hold committed tokens (clamped to [0, max_blocks *
+ * block_size]).  block_size: a power of two, at least 8.  type: PZ_BF16 or
+ * PZ_F16.  head_dim: 64, 128 or 256.  ld a multiple of 8, d_k and d_v 16-byte
+ * aligned.  A page number outside [0, n_blocks) holds no positions: reading
+ * leaves them out, as if they were masked, and writing skips them. */
+typedef struct {
+  int type;
+  int n_kv_heads;
+  int head_dim;
+  void *d_k;
+  void *d_v;
+  long ld;
+  int n_blocks;
+  int block_size;
+  const int32_t *d_blocks;
+  int max_blocks;
+  const int32_t *d_len;
+} pz_kv_cache;
+
+/* Attention of drafted tokens over a cache and over each other.  Sequence b
+ * has n_b = min(d_n_nodes[b], T) nodes (d_n_nodes NULL: T; T <=
+ * PZ_TREE_MAX_NODES) whose keys and values are not in the cache yet: node t's
+ * at d_kn + (b * T + t) * ld_n (n_kv_heads x head_dim elements of the cache's
+ * type), and d_vn alike.  Node t attends the d_len[b] cached positions and
+ * every node u < n_b with bit u set in d_tree[b * T + t] (itself only if its
+ * own bit is set); d_tree NULL is a chain, node t attending nodes 0 .. t (a
+ * target forward over drafts; T = 1: decoding).  For head h of n_heads, with
+ * key head h / (n_heads / n_kv_heads):
+ *   out[b, t, h] = sum_p softmax_p(scale * q[b, t, h] . k[p]) v[p]
+ * q row (b, t) at d_q + (b * T + t) * ld_q, n_heads x head_dim elements; out
+ * alike with ld_out.  Sums and softmax in fp32; softmax weights are rounded
+ * to the type before they meet the values, the result once more.  A node that
+ * attends nothing gets zeros; what a node does not attend has no influence,
+ * NaN included; rows of nodes from n_b on are left as they are.  ld_q, ld_n
+ * and ld_out multiples of 8, pointers 16-byte aligned.  Long sequences are
+ * split over workgroups, in a workspace that the first call allocates (64 MiB,
+ * kept until the sampler is destroyed).
+ * Asynchronous on the sampler's stream; after that first call it can be
+ * captured into a HIP graph.  Calls of one sampler, replays included, must be
+ * ordered (on one stream or by events): they share the workspace. */
+#define PZ_TREE_MAX_NODES 64
+PZ_API int pz_tree_attention(pz_sampler *s, const pz_kv_cache *cache, const void *d_kn,
+                             const void *d_vn, long ld_n, int B, int T,
+                             const int32_t *d_n_nodes, const uint64_t *d_tree, int n_heads,
+                             float scale, const void *d_q, long ld_q, void *d_out, long ld_out);
+
+/* Appends accepted nodes to the cache: for every sequence b and i <
+ * min(d_count[b], T), the keys and values of node d_take[b * T + i] go to
+ * position d_len[b] + i (d_take NULL: node i; d_count NULL: T).  A node
+ * outside [0, T), a position past the table and a page outside the cache are
+ * skipped.  d_len is read, not advanced.  d_kn, d_vn, ld_n as
+ * pz_tree_attention.  Asynchronous on the sampler's stream. */
+PZ_API int pz_cache_append(pz_sampler *s, const pz_kv_cache *cache, const void *d_kn,
+                           const void *d_vn, long ld_n, int B, int T, const int32_t *d_take,
+                           const int32_t *d_count);
 
 /* Device memory helpers for C hosts (hipMalloc / hipFree / hipMemcpy). */
 PZ_API int pz_device_alloc(void **ptr, size_t bytes, int device);

@@ -38,6 +38,7 @@
 
 #include "../../include/pz_sampler.h"
 #include "pz_device.h"
+#include "pz_lmdev.h"
 #include "pz_lmtile.h"
 #include "pz_sampler_impl.h"
 
@@ -51,18 +52,12 @@ constexpr size_t LM_LDS_MAX = 96 * 1024;        // x tile budget
 
 // The 8 weights of one 16-byte load (little-endian: element 2k is the low
 // half of word k).
-typedef uint32_t lm_u32x4 __attribute__((ext_vector_type(4)));
-typedef float lm_f32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void widen8(const lm_u32x4 q, float (&w)[8]) {
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     w[2 * i] = __uint_as_float(q[i] << 16);
     w[2 * i + 1] = __uint_as_float(q[i] & 0xffff0000u);
   }
-}
-
-__device__ __forceinline__ uint64_t argmax_key(float v, int id) {
-  return ((uint64_t)pz_key(v) << 32) | (uint64_t)(0xffffffffu - (uint32_t)id);
 }
 
 // MODE 0: write logits.  MODE 1: argmax keys.  VEC: n % 8 == 0 and W 16-byte
@@ -238,11 +233,6 @@ constexpr int LMX_FRAG = 512;  // bf16 of one fragment (16 x 32)
 
 __device__ __forceinline__ float lm_bf16_f(uint16_t h) { return __uint_as_float((uint32_t)h << 16); }
 
-// Keys of the fused argmax spread over LMM_SLOTS slots per batch row (one
-// per workgroup index modulo LMM_SLOTS, each on its own cache line), so the
-// workgroups' atomics do not all meet on the batch's few words.
-constexpr int LMM_SLOTS = 16;
-
 // The three bf16 parts of 8 activations, two to a word.
 __device__ __forceinline__ void lm_split8(const float (&x)[8], lm_u32x4 (&h)[3]) {
 #pragma unroll
@@ -277,34 +267,6 @@ __global__ __launch_bounds__(64) void k_lmx_split(const float* __restrict__ X, l
 #pragma unroll
   for (int p = 0; p < 3; p++)
     *reinterpret_cast<lm_u32x4*>(o + p * LMX_FRAG) = h[p];
-}
-
-// 16 bytes per lane from base + off to LDS at byte address lds + 16 lane.
-// (Written as asm because for the builtin the compiler orders every later
-// LDS read of the workgroup behind all such loads; the stage loop below
-// waits for exactly the loads that it needs.  M0, the LDS base, is a clobber:
-// a value that the compiler keeps there is not taken for one that survived.)
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"  // (M0 is a reserved register)
-template <bool NT>
-__device__ __forceinline__ void lm_lds_load16(const void* base, uint32_t off, uint32_t lds) {
-  if (NT)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt"
-                 :
-                 : "s"(lds), "v"(off), "s"(base)
-                 : "m0", "memory");
-  else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                 :
-                 : "s"(lds), "v"(off), "s"(base)
-                 : "m0", "memory");
-}
-#pragma clang diagnostic pop
-// At most N of this wave's vector memory operations, and none of its LDS
-// operations, still outstanding.
-template <int N>
-__device__ __forceinline__ void lm_wait() {
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(N) : "memory");
 }
 
 template <int WR, int WC, int TR, int TC, int KS, int NS, int MODE, bool NT>
@@ -761,6 +723,13 @@ int check(pz_sampler* s, const uint16_t* d_w, int V, int n, const float* d_x, in
 
 }  // namespace
 
+int pz_lm_finish(pz_sampler* s, int B, int32_t* d_ids) {
+  hipLaunchKernelGGL(k_lmhead_finish, dim3((B + 255) / 256), dim3(256), 0, s->stream, B,
+                     s->d_lmh_keys, s->max_batch, s->d_lmh_nan, d_ids);
+  PZ_HIP(s, hipGetLastError());
+  return PZ_OK;
+}
+
 extern "C" int pz_lm_head_bf16(pz_sampler* s, const uint16_t* d_w, int V, int n, const float* d_x,
                                int B, long ldx, float* d_logits, long ld) {
   if (!s) return PZ_EINVAL;
@@ -782,8 +751,5 @@ extern "C" int pz_lm_head_argmax_bf16(pz_sampler* s, const uint16_t* d_w, int V,
   PZ_HIP(s, hipSetDevice(s->device));
   const int r = run<1>(s, d_w, V, n, d_x, B, ldx, nullptr, 0);
   if (r != PZ_OK) return r;
-  hipLaunchKernelGGL(k_lmhead_finish, dim3((B + 255) / 256), dim3(256), 0, s->stream, B,
-                     s->d_lmh_keys, s->max_batch, s->d_lmh_nan, d_ids);
-  PZ_HIP(s, hipGetLastError());
-  return PZ_OK;
+  return pz_lm_finish(s, B, d_ids);
 }

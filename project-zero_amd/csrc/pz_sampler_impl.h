@@ -10,6 +10,7 @@
 #include "pz_params.h"
 
 constexpr int PZ_LMX_ROWS = 256;  // batch rows of one LM-head GEMM launch
+constexpr size_t PZ_TREE_WS = (size_t)64 << 20;  // bytes of tree attention's workspace
 
 struct pz_sampler {
   int device = 0;
@@ -60,6 +61,10 @@ struct pz_sampler {
   // more): lmh_x_elems bf16, PZ_LMX_ROWS batch rows of n = 8192
   uint16_t* d_lmh_x = nullptr;
   size_t lmh_x_elems = 0;
+
+  // tree attention's partial results (PZ_TREE_WS bytes, allocated by its first
+  // call and kept, so captured calls stay valid)
+  void* tree_dev = nullptr;
 
   const float* call_u = nullptr;  // the synchronous call's host uniforms, during the call
 
@@ -147,6 +152,10 @@ int pz_launch_softmax_rows(pz_sampler* s, const float* d_in, long ld_in, float* 
 int pz_launch_softmax_split(pz_sampler* s, const PzSplitWs& ws, const float* d_in, long ld_in,
                             float* d_out, long ld_out, int n_rows, int n, PzTemp T,
                             const int32_t* d_len);
+
+// Ids from the fused LM heads' argmax keys (s->d_lmh_keys, s->d_lmh_nan),
+// which it clears for the next call.
+int pz_lm_finish(pz_sampler* s, int B, int32_t* d_ids);
 
 // Launches the kernels for B rows whose kernel parameters are already in
 // s->res_params (n_params entries).  Used by the public entry points after

@@ -17,6 +17,9 @@ SYNTH_LIB = os.path.join(LIB_DIR, "libpzsynth.so")
 
 PZ_OK, PZ_EINVAL, PZ_ENOMEM, PZ_EDEVICE, PZ_ERANGE, PZ_ENOTSUP = 0, -1, -2, -3, -4, -5
 PZ_TEMP_MUL_RECIP, PZ_TEMP_DIV = 0, 1
+PZ_F32, PZ_BF16, PZ_F16 = 0, 1, 2
+PZ_I8_MAX_N = 131071
+PZ_TREE_MAX_NODES = 64
 
 # Every symbol include/pz_sampler.h and include/pz_sampling_compat.h declare.
 ABI_SYMBOLS = (
@@ -28,6 +31,8 @@ ABI_SYMBOLS = (
     "pz_sample_step", "pz_sampler_set_eos", "pz_attn_softmax", "pz_lm_head_bf16",
     "pz_lm_head_argmax_bf16", "pz_spec_decode", "pz_sampler_set_wait_bound",
     "pz_spec_verify_greedy", "pz_spec_verify_greedy_async", "pz_spec_decode_opts",
+    "pz_rules_batch", "pz_quant_rows_i8", "pz_lm_head_i8", "pz_lm_head_argmax_i8",
+    "pz_tree_attention", "pz_cache_append",
     # include/pz_sampling_compat.h: the reference sampler's own symbols
     "sample_argmax", "apply_temperature", "sample_top_p", "sample_top_k", "rng_seed",
     "rng_float", "pz_tn_softmax", "pz_compat_set_temp_mode", "pz_compat_last_status",
@@ -55,6 +60,65 @@ def row_params(temperature=1.0, top_k=0, top_p=1.0, rep_penalty=1.0,
                presence_penalty=0.0, frequency_penalty=0.0):
     return RowParams(temperature, top_k, top_p, rep_penalty, presence_penalty,
                      frequency_penalty)
+
+
+class LogitRules(ctypes.Structure):
+    _fields_ = [
+        ("rep_penalty", ctypes.c_float),
+        ("presence_penalty", ctypes.c_float),
+        ("frequency_penalty", ctypes.c_float),
+        ("d_penalties", ctypes.c_void_p),
+        ("d_hist", ctypes.c_void_p),
+        ("H", ctypes.c_int),
+        ("d_hist_len", ctypes.c_void_p),
+        ("d_bias_ids", ctypes.c_void_p),
+        ("d_bias", ctypes.c_void_p),
+        ("n_bias", ctypes.c_int),
+        ("d_mask", ctypes.c_void_p),
+        ("ld_mask", ctypes.c_long),
+        ("n_masks", ctypes.c_int),
+        ("d_mask_row", ctypes.c_void_p),
+        ("d_allowed", ctypes.c_void_p),
+    ]
+
+
+class KvCache(ctypes.Structure):
+    _fields_ = [
+        ("type", ctypes.c_int),
+        ("n_kv_heads", ctypes.c_int),
+        ("head_dim", ctypes.c_int),
+        ("d_k", ctypes.c_void_p),
+        ("d_v", ctypes.c_void_p),
+        ("ld", ctypes.c_long),
+        ("n_blocks", ctypes.c_int),
+        ("block_size", ctypes.c_int),
+        ("d_blocks", ctypes.c_void_p),
+        ("max_blocks", ctypes.c_int),
+        ("d_len", ctypes.c_void_p),
+    ]
+
+
+def _filled(struct, kw):
+    """struct with its device buffers (d_*) by address; it keeps them alive."""
+    names = {n for n, _ in struct._fields_}
+    for k, v in kw.items():
+        if k not in names:
+            raise TypeError(f"{struct.__name__} has no field {k}")
+    r = struct(**{k: _ptr(v) if k.startswith("d_") else v for k, v in kw.items()})
+    r.buffers = [v for k, v in kw.items() if k.startswith("d_")]
+    return r
+
+
+def logit_rules(rep_penalty=1.0, presence_penalty=0.0, frequency_penalty=0.0, **kw):
+    """pz_logit_rules; device buffers as addresses or torch tensors."""
+    return _filled(LogitRules, dict(kw, rep_penalty=rep_penalty,
+                                    presence_penalty=presence_penalty,
+                                    frequency_penalty=frequency_penalty))
+
+
+def kv_cache(**kw):
+    """pz_kv_cache; device buffers as addresses or torch tensors."""
+    return _filled(KvCache, kw)
 
 
 _lib = None
@@ -110,6 +174,13 @@ def load():
     lib.pz_spec_verify_greedy.argtypes = [_P, _P, _I, _I, _I, _L, _I, _F, _P, _P, _P, _P, _P]
     lib.pz_spec_verify_greedy_async.argtypes = [_P, _P, _I, _I, _I, _L, _I, _F, _P, _P, _P,
                                                 _P, _P]
+    lib.pz_rules_batch.argtypes = [_P, _P, _L, _P, _L, _I, _I, ctypes.POINTER(LogitRules)]
+    lib.pz_quant_rows_i8.argtypes = [_P, _P, _I, _L, _I, _I, _P, _L, _P]
+    lib.pz_lm_head_i8.argtypes = [_P, _P, _P, _I, _I, _P, _P, _I, _L, _P, _L]
+    lib.pz_lm_head_argmax_i8.argtypes = [_P, _P, _P, _I, _I, _P, _P, _I, _L, _P]
+    lib.pz_tree_attention.argtypes = [_P, ctypes.POINTER(KvCache), _P, _P, _L, _I, _I, _P, _P, _I,
+                                      _F, _P, _L, _P, _L]
+    lib.pz_cache_append.argtypes = [_P, ctypes.POINTER(KvCache), _P, _P, _L, _I, _I, _P, _P]
     pull = ctypes.POINTER(ctypes.c_ulonglong)
     lib.sample_argmax.argtypes = [_P, _I]
     lib.apply_temperature.argtypes = [_P, _I, _F]
@@ -302,6 +373,47 @@ class Sampler:
         _sync_torch(d_w, d_x, d_ids)
         self._check(self.lib.pz_lm_head_argmax_bf16(self.h, _ptr(d_w), V, n, _ptr(d_x), B, ldx,
                                                     _ptr(d_ids)))
+
+    def rules(self, d_in, d_out, B, V, ld_in, ld_out, rules):
+        """Penalties, biases and masks of logit_rules(...) applied to B rows,
+        in place when d_out is d_in (asynchronous)."""
+        _sync_torch(d_in, d_out)
+        self._check(self.lib.pz_rules_batch(self.h, _ptr(d_in), ld_in, _ptr(d_out), ld_out, B, V,
+                                            ctypes.byref(rules)))
+
+    def quant_rows_i8(self, d_x, x_type, ldx, rows, n, d_q, ldq, d_scale):
+        """Rows of x_type to int8 with a scale each (asynchronous)."""
+        _sync_torch(d_x, d_q, d_scale)
+        self._check(self.lib.pz_quant_rows_i8(self.h, _ptr(d_x), x_type, ldx, rows, n, _ptr(d_q),
+                                              ldq, _ptr(d_scale)))
+
+    def lm_head_i8(self, d_w, d_sw, V, n, d_x, d_sx, B, ldx, d_logits, ld):
+        """logits[b, i] = (W[i, :] . x[b, :]) * sw[i] * sx[b], int8 operands
+        (asynchronous)."""
+        _sync_torch(d_w, d_x, d_logits)
+        self._check(self.lib.pz_lm_head_i8(self.h, _ptr(d_w), _ptr(d_sw), V, n, _ptr(d_x),
+                                           _ptr(d_sx), B, ldx, _ptr(d_logits), ld))
+
+    def lm_head_argmax_i8(self, d_w, d_sw, V, n, d_x, d_sx, B, ldx, d_ids):
+        """Greedy ids of the 8-bit LM head's logits, argmax fused (asynchronous)."""
+        _sync_torch(d_w, d_x, d_ids)
+        self._check(self.lib.pz_lm_head_argmax_i8(self.h, _ptr(d_w), _ptr(d_sw), V, n, _ptr(d_x),
+                                                  _ptr(d_sx), B, ldx, _ptr(d_ids)))
+
+    def tree_attention(self, cache, d_kn, d_vn, ld_n, B, T, n_heads, scale, d_q, ld_q, d_out,
+                       ld_out, d_n_nodes=None, d_tree=None):
+        """Attention of T nodes per sequence over kv_cache(...) and along the
+        tree, d_tree None: a chain (asynchronous)."""
+        _sync_torch(d_q, d_kn, d_out)
+        self._check(self.lib.pz_tree_attention(
+            self.h, ctypes.byref(cache), _ptr(d_kn), _ptr(d_vn), ld_n, B, T, _ptr(d_n_nodes),
+            _ptr(d_tree), n_heads, scale, _ptr(d_q), ld_q, _ptr(d_out), ld_out))
+
+    def cache_append(self, cache, d_kn, d_vn, ld_n, B, T, d_take=None, d_count=None):
+        """Accepted nodes' keys and values into the cache's pages (asynchronous)."""
+        _sync_torch(d_kn, d_vn)
+        self._check(self.lib.pz_cache_append(self.h, ctypes.byref(cache), _ptr(d_kn), _ptr(d_vn),
+                                             ld_n, B, T, _ptr(d_take), _ptr(d_count)))
 
     def spec_verify(self, d_target, d_draft, B, K, V, ld, has_bonus, temperature,
                     draft_ids, u_acc, u_res):
