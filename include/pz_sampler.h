@@ -391,8 +391,8 @@ typedef struct {
 
 /* Applies the rules to B rows of V logits: d_out[r, i] from d_in[r, i], bit
  * for bit as above in fp32.  d_out == d_in (with ld_out == ld_in) works in
- * place, which writes only the ids that a rule names and those the mask rules
- * out; otherwise the two must not overlap, and every d_out[r, 0 .. V) is
+ * place and touches only the groups of four ids in which a rule names or rules
+ * out one; otherwise the two must not overlap, and every d_out[r, 0 .. V) is
  * written.  For the samplers' rows and for verification's (B * (K + 1) rows,
  * each with its own history); no limit by the sampler's max_batch, max_vocab
  * or max_hist.  Reads *rules during the call only.  Asynchronous on the

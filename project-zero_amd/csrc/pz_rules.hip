@@ -6,17 +6,19 @@
 //   y = in[i]; c > 0: y = (y > 0 ? y / rep : y * rep) - (c * freq + pres)
 //   (the samplers' own penalties, pz_penalize); y += bias, entry by entry;
 //   masked ids: -infinity.
-// Integer atomics only, so the order in which ids arrive changes nothing; two
-// bias entries of one id are added by one thread in the list's order.
+// Integer atomics only, so the order in which ids arrive changes nothing; the
+// bias entries of one id are added in the list's order.
 //
 //   * A row is cut into slices of W ids, one workgroup each; a workgroup reads
 //     the whole history and keeps the ids of its slice.  In place and without
 //     masks only the named ids are touched: one slice, a hash table of twice
 //     the entries.  Lists too long for that take a table indexed by the id
-//     itself (DENSE), 8192 ids a slice.
-//   * With masks, or out of place, the slice's ids also stream through: four
-//     ids a thread, a mask nibble, one 16-byte store where anything changes.
-//     In place, nothing of an all-allowed group is read or written.
+//     itself (DENSE).
+//   * With masks, or out of place, the slice's ids also stream through: 4 NQ
+//     ids a thread, all loads of them issued before the table is made, the
+//     slice's mask words in LDS, one 16-byte store where anything changes.  In
+//     place, nothing of an all-allowed group is read or written.
+//   * d_allowed has a workgroup of its own per row, beside the slices.
 #include <hip/hip_runtime.h>
 
 #include "../../include/pz_sampler.h"
@@ -26,14 +28,17 @@
 
 namespace {
 
-constexpr int RU_NONE = 0x7fffffff;  // no bias entry
+constexpr int RU_NONE = 0x7fffffff;         // no bias entry
+constexpr uint32_t RU_TWICE = 0x80000000u;  // in a count (DENSE): the id has more bias entries
+constexpr int RU_WALK = 12;                 // entries of one id that its thread walks through itself
 
 struct RulesArgs {
   const float* in;
   long ld_in;
   float* out;
   long ld_out;
-  int V, W, S, cap;  // ids, ids of a slice, slices of a row, hash entries
+  int V, W, S, cap;  // ids, ids of a slice, slices of a row, slots of a table
+  int count;         // 1: a workgroup more per row counts what its mask allows
   pz_logit_rules r;
 };
 
@@ -46,13 +51,16 @@ __device__ __forceinline__ const uint32_t* ru_mask(const pz_logit_rules& r, int 
   return m >= 0 && m < r.n_masks ? r.d_mask + (size_t)m * r.ld_mask : nullptr;
 }
 
-// The table: per slot the count and the first bias entry, and with !DENSE the
-// id (-1: empty).
+// The table: per slot the count and a bias entry (DENSE: the first, and a mark
+// in the count where there are more; else the last to arrive, the others
+// chained to it), and with !DENSE the id (-1: empty).
 template <bool DENSE>
 struct RuTable {
   uint32_t* cnt;
   int32_t* first;
   int32_t* key;
+  int32_t* used;  // (!DENSE) the slots taken, in no order, and how many
+  int* n_used;
   int base, lim, cap;
   __device__ __forceinline__ int slot(int id) const {
     if (DENSE) return id - base;
@@ -61,29 +69,88 @@ struct RuTable {
     // at most half of the slots are ever taken, so an empty one ends this
     while (true) {
       const int prev = atomicCAS(&key[s], -1, id);
+      if (prev == -1) used[atomicAdd(n_used, 1)] = (int)s;
       if (prev == -1 || prev == id) return (int)s;
       s = (s + 1) & mask;
     }
   }
 };
 
-template <bool DENSE, bool STREAM, int BLOCK>
+// The number of ids that a mask allows, by one workgroup.
+template <int BLOCK>
+__device__ __forceinline__ int ru_count(const uint32_t* mask, int V) {
+  __shared__ int n_on;
+  if (threadIdx.x == 0) n_on = 0;
+  __syncthreads();
+  int n = 0;
+  const int words = (V + 31) >> 5;
+#pragma unroll 4
+  for (int w = threadIdx.x; w < words; w += BLOCK) {
+    const uint32_t tail = w == words - 1 && (V & 31) ? (1u << (V & 31)) - 1u : ~0u;
+    n += __popc(mask[w] & tail);
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
+  if ((threadIdx.x & 63) == 0) atomicAdd(&n_on, n);
+  __syncthreads();
+  return n_on;
+}
+
+// NQ 0: only the named ids that the mask allows.
+template <bool DENSE, int NQ, int BLOCK>
 __global__ __launch_bounds__(BLOCK) void k_rules(const RulesArgs A) {
+  constexpr int U = 4;  // slots of a thread whose logits are on their way together
   extern __shared__ __align__(16) char lds[];
-  __shared__ int dup, n_on;
+  __shared__ uint32_t on_sh[NQ ? NQ * BLOCK / 8 : 1];
+  __shared__ int n_used;
   const pz_logit_rules& r = A.r;
-  const int tid = threadIdx.x;
-  const int b = blockIdx.x / A.S, sl = blockIdx.x - b * A.S;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int per = A.S + A.count;
+  const int b = blockIdx.x / per, sl = blockIdx.x - b * per;
   const int V = A.V;
+  // (the first of the history while the mask and the parameters arrive)
+  const int32_t* h = r.d_hist + (size_t)b * r.H;
+  ru_i4u h0;
+  if (4 * tid + 3 < r.H) h0 = *reinterpret_cast<const ru_i4u*>(h + 4 * tid);
+  const uint32_t* mask = ru_mask(r, b);
+  if (sl == A.S) {
+    const int n = mask ? ru_count<BLOCK>(mask, V) : V;
+    if (tid == 0) r.d_allowed[b] = n;
+    return;
+  }
   RuTable<DENSE> T;
   T.base = sl * A.W;
   T.lim = V - T.base < A.W ? V : T.base + A.W;
-  T.cap = DENSE ? A.W : A.cap;
+  T.cap = A.cap;
   T.cnt = reinterpret_cast<uint32_t*>(lds);
   T.first = reinterpret_cast<int32_t*>(lds) + T.cap;
   T.key = reinterpret_cast<int32_t*>(lds) + 2 * T.cap;
+  T.used = T.key + T.cap;  // (at most half of the slots)
+  T.n_used = &n_used;
+  // (!DENSE) the entry that named an entry's id before it
+  int32_t* next = T.used + T.cap / 2;
   const float* in = A.in + (size_t)b * A.ld_in;
   float* out = A.out + (size_t)b * A.ld_out;
+  const bool inplace = A.in == A.out;
+  pz_f4u q[NQ ? NQ : 1];
+  if constexpr (NQ > 0) {
+    if (!inplace) {
+#pragma unroll
+      for (int k = 0; k < NQ; k++) {
+        const int i = T.base + 4 * (k * BLOCK + tid);
+        if (i + 3 < T.lim) {
+          q[k] = *reinterpret_cast<const pz_f4u*>(in + i);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; e++) q[k][e] = i + e < T.lim ? in[i + e] : 0.0f;
+        }
+      }
+    }
+    if (mask)
+#pragma unroll
+      for (int w = tid; w < NQ * BLOCK / 8; w += BLOCK)
+        on_sh[w] = T.base + 32 * w < T.lim ? mask[(T.base >> 5) + w] : 0u;
+  }
   float rep = r.rep_penalty, pres = r.presence_penalty, freq = r.frequency_penalty;
   if (r.d_penalties) {
     rep = r.d_penalties[3 * (size_t)b];
@@ -96,8 +163,9 @@ __global__ __launch_bounds__(BLOCK) void k_rules(const RulesArgs A) {
     H = n < 0 ? 0 : (n < H ? n : H);
   }
   if (rep == 1.0f && pres == 0.0f && freq == 0.0f) H = 0;
-  const uint32_t* mask = ru_mask(r, b);
   const bool lists = H > 0 || r.n_bias > 0;
+  const int32_t* bid = r.d_bias_ids + (size_t)b * r.n_bias;
+  const float* bias = r.d_bias + (size_t)b * r.n_bias;
 
   if (lists) {
     for (int i = tid; i < T.cap; i += BLOCK) {
@@ -105,98 +173,139 @@ __global__ __launch_bounds__(BLOCK) void k_rules(const RulesArgs A) {
       T.first[i] = RU_NONE;
       if (!DENSE) T.key[i] = -1;
     }
-    if (tid == 0) dup = 0;
+    if (tid == 0) n_used = 0;
     __syncthreads();
-    const int32_t* h = r.d_hist + (size_t)b * r.H;
     auto seen = [&](int id) {
       if (id >= T.base && id < T.lim) atomicAdd(&T.cnt[T.slot(id)], 1u);
     };
     const int H4 = H & ~3;
-    for (int j = 4 * tid; j < H4; j += 4 * BLOCK) {
-      const ru_i4u q = *reinterpret_cast<const ru_i4u*>(h + j);
+    if (4 * tid < H4)
 #pragma unroll
-      for (int e = 0; e < 4; e++) seen(q[e]);
+      for (int e = 0; e < 4; e++) seen(h0[e]);
+    int j = 4 * (BLOCK + tid);
+    for (; j < H4 - 12 * BLOCK; j += 16 * BLOCK) {  // (four loads on their way)
+      ru_i4u h4[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        h4[k] = *reinterpret_cast<const ru_i4u*>(h + j + 4 * k * BLOCK);
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) seen(h4[k][e]);
     }
-    for (int j = H4 + tid; j < H; j += BLOCK) seen(h[j]);
-    const int32_t* bid = r.d_bias_ids + (size_t)b * r.n_bias;
+    for (; j < H4; j += 4 * BLOCK) {
+      const ru_i4u h4 = *reinterpret_cast<const ru_i4u*>(h + j);
+#pragma unroll
+      for (int e = 0; e < 4; e++) seen(h4[e]);
+    }
+    for (j = H4 + tid; j < H; j += BLOCK) seen(h[j]);
     for (int e = tid; e < r.n_bias; e += BLOCK) {
       const int id = bid[e];
-      if (id >= T.base && id < T.lim && atomicMin(&T.first[T.slot(id)], e) != RU_NONE) dup = 1;
+      if (id < T.base || id >= T.lim) continue;
+      const int at = T.slot(id);
+      if (!DENSE) next[e] = atomicExch(&T.first[at], e);
+      else if (atomicMin(&T.first[at], e) != RU_NONE) atomicOr(&T.cnt[at], RU_TWICE);
     }
   }
-  if (STREAM) {
-    const bool inplace = A.in == A.out;
+  if constexpr (NQ > 0) {
+    if (mask && !lists) __syncthreads();
+    // (with lists, the barrier after the tables were cleared)
     const float ninf = -__builtin_inff();
-    if (!inplace || mask)
-      for (int i = T.base + 4 * tid; i < T.lim; i += 4 * BLOCK) {
-        const uint32_t on = mask ? mask[i >> 5] >> (i & 31) & 0xfu : 0xfu;
-        if (inplace && on == 0xfu) continue;
-        if (i + 3 < T.lim) {
-          pz_f4u q;
-          if (!inplace) q = *reinterpret_cast<const pz_f4u*>(in + i);
-          if (!inplace || on == 0u) {
+    uint32_t on[NQ];
 #pragma unroll
-            for (int e = 0; e < 4; e++) q[e] = on >> e & 1u ? q[e] : ninf;
-            *reinterpret_cast<pz_f4u*>(out + i) = q;
-          } else {
+    for (int k = 0; k < NQ; k++) {
+      const int t = k * BLOCK + tid, i = T.base + 4 * t;
+      on[k] = mask ? on_sh[t >> 3] >> (4 * (t & 7)) & 0xfu : 0xfu;
+      if (inplace && on[k] != 0xfu && on[k] != 0u && i + 3 < T.lim)
+        q[k] = *reinterpret_cast<const pz_f4u*>(in + i);
+    }
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-              if (!(on >> e & 1u)) out[i + e] = ninf;
-          }
-        } else {
-          for (int e = 0; i + e < T.lim; e++) {
-            if (!(on >> e & 1u)) out[i + e] = ninf;
-            else if (!inplace) out[i + e] = in[i + e];
+    for (int k = 0; k < NQ; k++) {
+      const int i = T.base + 4 * (k * BLOCK + tid);
+      if (inplace && on[k] == 0xfu) continue;
+      if (i + 3 < T.lim) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) q[k][e] = on[k] >> e & 1u ? q[k][e] : ninf;
+        *reinterpret_cast<pz_f4u*>(out + i) = q[k];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const bool keep = on[k] >> e & 1u;
+          if (i + e < T.lim && !(inplace && keep)) out[i + e] = keep ? q[k][e] : ninf;
+        }
+      }
+    }
+  }
+  if (!lists) return;
+  __syncthreads();  // the table is complete, and so is the slice's stream
+  const int slots = DENSE ? T.cap : n_used;
+  for (int i0 = 0; i0 < slots; i0 += U * BLOCK) {
+    uint32_t c[U];
+    int f[U], id[U];
+    float x[U], bv[U];
+    bool act[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int at = i0 + u * BLOCK + tid;
+      c[u] = 0u;
+      f[u] = RU_NONE;
+      id[u] = 0;
+      if (at < slots) {
+        const int i = DENSE ? at : T.used[at];
+        c[u] = T.cnt[i];
+        f[u] = T.first[i];
+        id[u] = DENSE ? T.base + i : T.key[i];
+      }
+      act[u] = c[u] != 0u || f[u] != RU_NONE;
+      if (act[u] && mask)
+        act[u] = (NQ ? on_sh[(id[u] - T.base) >> 5] : mask[id[u] >> 5]) >> (id[u] & 31) & 1u;
+      x[u] = bv[u] = 0.0f;
+      if (act[u]) x[u] = in[id[u]];
+      if (act[u] && f[u] != RU_NONE) bv[u] = bias[f[u]];
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const uint32_t times = c[u] & ~RU_TWICE;
+      if (act[u] && times) {
+        x[u] = x[u] > 0.0f ? x[u] / rep : x[u] * rep;
+        float t = (float)times * freq;
+        t = t + pres;
+        x[u] = x[u] - t;
+      }
+      bool many = act[u] && (c[u] & RU_TWICE);
+      if (act[u] && f[u] != RU_NONE && !many) {
+        int n = 1;
+        if (!DENSE)
+          for (int e = next[f[u]]; e != RU_NONE && n <= RU_WALK; e = next[e]) n++;
+        many = n > RU_WALK;
+        if (n == 1) {
+          x[u] = x[u] + bv[u];
+        } else if (!many) {
+          // a short chain, in no order: its entries in the list's order
+          for (int last = -1, k = 0; k < n; k++) {
+            int lo = RU_NONE;
+            for (int e = f[u]; e != RU_NONE; e = next[e]) lo = e > last && e < lo ? e : lo;
+            x[u] = x[u] + bias[lo];
+            last = lo;
           }
         }
       }
-  }
-  if (lists) {
-    __syncthreads();  // the table is complete, and so is the slice's stream
-    const int32_t* bid = r.d_bias_ids + (size_t)b * r.n_bias;
-    const float* bias = r.d_bias + (size_t)b * r.n_bias;
-    const bool twice = dup != 0;
-    for (int i = tid; i < T.cap; i += BLOCK) {
-      const uint32_t c = T.cnt[i];
-      const int f = T.first[i];
-      if (c == 0u && f == RU_NONE) continue;
-      const int id = DENSE ? T.base + i : T.key[i];
-      if (mask && !(mask[id >> 5] >> (id & 31) & 1u)) continue;
-      float x = in[id];
-      if (c) {
-        x = x > 0.0f ? x / rep : x * rep;
-        float t = (float)c * freq;
-        t = t + pres;
-        x = x - t;
+      // an id with many entries: the wave looks through the list
+      for (uint64_t todo = __ballot(many); todo; todo &= todo - 1) {
+        const int L = __builtin_ctzll(todo);
+        const int its = __builtin_amdgcn_readlane(id[u], L);
+        float v = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x[u]), L));
+        for (int e0 = 0; e0 < r.n_bias; e0 += 64) {
+          const int e = e0 + lane;
+          const bool is = e < r.n_bias && bid[e] == its;
+          const int more = is ? __float_as_int(bias[e]) : 0;
+          for (uint64_t hit = __ballot(is); hit; hit &= hit - 1)
+            v = v + __int_as_float(__builtin_amdgcn_readlane(more, __builtin_ctzll(hit)));
+        }
+        if (lane == L) x[u] = v;
       }
-      if (f != RU_NONE) {
-        x = x + bias[f];
-        if (twice)
-          for (int e = f + 1; e < r.n_bias; e++)
-            if (bid[e] == id) x = x + bias[e];
-      }
-      out[id] = x;
+      if (act[u]) out[id[u]] = x[u];
     }
-  }
-  if (r.d_allowed && sl == 0) {
-    // (the row's first workgroup counts all of it)
-    if (!mask) {
-      if (tid == 0) r.d_allowed[b] = V;
-      return;
-    }
-    if (tid == 0) n_on = 0;
-    __syncthreads();
-    int n = 0;
-    const int words = (V + 31) >> 5;
-    for (int w = tid; w < words; w += BLOCK) {
-      const uint32_t tail = w == words - 1 && (V & 31) ? (1u << (V & 31)) - 1u : ~0u;
-      n += __popc(mask[w] & tail);
-    }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
-    if ((tid & 63) == 0) atomicAdd(&n_on, n);
-    __syncthreads();
-    if (tid == 0) r.d_allowed[b] = n_on;
   }
 }
 
@@ -206,16 +315,20 @@ int next_pow2(long v) {
   return p;
 }
 
-constexpr int RU_HASH_MOST = 2048;  // list entries a hash table is made for
-constexpr int RU_DENSE = 8192;      // ids of a slice with a table of its own
-
-template <bool DENSE, bool STREAM, int BLOCK>
-int launch(pz_sampler* s, const RulesArgs& A, int B, size_t lds) {
-  auto k = k_rules<DENSE, STREAM, BLOCK>;
-  if (lds > 65536)
+template <bool DENSE, int NQ, int BLOCK>
+int launch(pz_sampler* s, RulesArgs& A, int B, size_t slot_bytes) {
+  if (NQ > 0) A.W = 4 * BLOCK * NQ;
+  A.S = (A.V + A.W - 1) / A.W;
+  if (DENSE) A.cap = A.W;
+  const int64_t grid = (int64_t)B * (A.S + A.count);
+  if (grid > INT32_MAX) return fail(s, PZ_ERANGE, "B=%d rows of V=%d", B, A.V);
+  const size_t lds = (size_t)A.cap * slot_bytes + (DENSE ? 0 : (size_t)A.r.n_bias * 4);
+  // (the counting workgroups and the mask words have LDS of their own)
+  auto k = k_rules<DENSE, NQ, BLOCK>;
+  if (lds > 65536 - 4096)
     PZ_HIP(s, hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize,
                                   (int)lds));
-  hipLaunchKernelGGL(k, dim3((unsigned)B * (unsigned)A.S), dim3(BLOCK), lds, s->stream, A);
+  hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(BLOCK), lds, s->stream, A);
   PZ_HIP(s, hipGetLastError());
   return PZ_OK;
 }
@@ -237,15 +350,33 @@ extern "C" int pz_rules_batch(pz_sampler* s, const float* d_in, long ld_in, floa
   A.r = *rules;
   const bool stream = d_in != d_out || A.r.n_masks > 0;
   const long entries = (long)A.r.H + A.r.n_bias;
-  if (!stream && entries == 0 && !A.r.d_allowed) return PZ_OK;
-  const bool dense = entries > RU_HASH_MOST;
-  A.W = dense || stream ? RU_DENSE : (V + 31) / 32 * 32;
-  A.S = (V + A.W - 1) / A.W;
-  if ((long)B * A.S > INT32_MAX) return fail(s, PZ_ERANGE, "B=%d rows of V=%d", B, V);
-  A.cap = dense ? 0 : next_pow2(2 * entries);
-  const size_t lds = entries == 0 ? 0 : dense ? (size_t)A.W * 8 : (size_t)A.cap * 12;
+  A.count = A.r.d_allowed ? 1 : 0;
+  if (!stream && entries == 0 && !A.count) return PZ_OK;
   PZ_HIP(s, hipSetDevice(s->device));
-  if (dense) return stream ? launch<true, true, 1024>(s, A, B, lds)
-                           : launch<true, false, 1024>(s, A, B, lds);
-  return stream ? launch<false, true, 256>(s, A, B, lds) : launch<false, false, 256>(s, A, B, lds);
+  // few rows: smaller slices, so that every CU has some
+  const bool few = (int64_t)B * ((V + 8191) / 8192) < 2 * s->n_cu;
+  if (stream) {
+    // Lists of up to 1024 entries are applied by the slices that stream; longer
+    // ones by a launch after them, because their tables leave room for fewer
+    // workgroups of the stream (256 rows of 151936 out of place with masks: 69
+    // us at H = 512, 104 at 1984 where a launch of its own makes it 81; 64 of
+    // 128256 in place at H = 2048 22.8 and 17.9).
+    RulesArgs L = A;
+    if (entries > 1024) L.r.H = L.r.n_bias = L.cap = 0;
+    else L.cap = entries == 0 ? 0 : next_pow2(2 * entries);
+    const int rc = few ? launch<false, 2, 256>(s, L, B, 14) : launch<false, 8, 256>(s, L, B, 14);
+    if (rc != PZ_OK || entries <= 1024) return rc;
+    A.count = 0;
+  }
+  // A hash table takes 14 bytes a slot at two slots an entry and 4 bytes a bias:
+  // up to 4096 entries fit, and one workgroup reads a row's history, not one
+  // per slice (256 rows of 128256, H = 2049: 7 us, 72 with a table per slice).
+  if (entries > 4096) {
+    A.W = few ? 2048 : 8192;
+    return launch<true, 0, 512>(s, A, B, 8);
+  }
+  A.W = (V + 31) / 32 * 32;
+  A.cap = entries == 0 ? 0 : next_pow2(2 * entries);
+  // (H = 2048: 256 threads 10.7 us for one row, 13.0 for 256; 1024 5.1 and 7.1)
+  return entries <= 256 ? launch<false, 0, 256>(s, A, B, 14) : launch<false, 0, 1024>(s, A, B, 14);
 }
