@@ -51,3 +51,40 @@ inline bool lm_own_parts(int V, int n, int B, int n_cu) {
   if (V <= 256 * n_cu) return n <= 256;
   return n <= (lm_once(V, n) ? 768 : 1024);
 }
+
+// The 8-bit head's shapes (pz_lmhead_i8.hip): batch rows and rows of W of a
+// workgroup's tile, and the longest W, in rows per CU, that takes the shape
+// before the next of its batch rows does.  Few rows take small tiles whose waves
+// share k; every bound lies between two sizes at which the neighbours were
+// timed (us at 256 CUs, each with both): 16 batch rows 8000 x 4096 7.7 / 9.1,
+// 14000 x 2560 9.9 / 8.7; 32 4000 x 2560 4.7 / 5.6, 8000 x 4096 8.7 / 7.9, 14000 x
+// 2560 9.3 / 10.6, 22000 x 2560 12.7 / 11.7; 64 4000 x 2560 6.2 / 7.1, 8000 x 4096
+// 14.2 / 10.4 / 14.9, 14000 x 2560 13.8 / 11.2, 40000 x 2560 28.4 / 29.5, 50257 x
+// 1024 19.8 / 17.9 / 18.5, 128256 x 2560 83 / 67; 128 4000 x 2560 8.7 / 9.0, 8000 x
+// 4096 21.8 / 13.5 / 23.0, 22000 x 2560 24.8 / 19.6 / 23.3, 40000 x 2560 40.4 / 32.9;
+// 256 4000 x 2560 14.3 / 16.4, 8000 x 4096 25.2 / 27.2, 14000 x 2560 24.5 / 19.7 /
+// 23.9, 22000 x 2560 28.1 / 24.8 / 38.0, 50257 x 1024 47.9 / 44.0.  Shape 2 in place
+// of 1 from 5 batch rows: 64000 x 2560 8 rows 34.4 / 31.9, 16 37.0 / 33.5.
+struct I8Tile {
+  int cols, rows, most;
+};
+constexpr I8Tile I8_TILE_SHAPES[] = {
+    {16, 16, 40},   {16, 32, 160},  {16, 64, 0},    // (0 - 2)
+    {32, 16, 24},   {32, 32, 60},   {32, 128, 0},   // (3 - 5)
+    {64, 16, 24},   {64, 32, 40},   {64, 64, 180},  {64, 128, 280}, {64, 256, 0},    // (6 - 10)
+    {128, 16, 24},  {128, 32, 60},  {128, 64, 140}, {128, 256, 0},                   // (11 - 14)
+    {256, 16, 24},  {256, 32, 40},  {256, 64, 70},  {256, 128, 140}, {256, 256, 0}}; // (15 - 19)
+constexpr int I8_TILE_COUNT = sizeof(I8_TILE_SHAPES) / sizeof(I8_TILE_SHAPES[0]);
+
+inline int i8_tile_for(int V, int B, int n_cu) {
+  const int cols = B <= 16 ? 16 : B <= 32 ? 32 : B <= 64 ? 64 : B <= 128 ? 128 : 256;
+  // (more than 256 batch rows: as many more workgroups)
+  const double rows = (double)V * ((B + cols - 1) / cols) / n_cu;
+  for (int i = 0; i < I8_TILE_COUNT; i++) {
+    const I8Tile& t = I8_TILE_SHAPES[i];
+    if (t.cols != cols) continue;
+    if (i == 1 && B <= 4) return i;
+    if (t.most == 0 || rows <= t.most) return i;
+  }
+  return I8_TILE_COUNT - 1;
+}

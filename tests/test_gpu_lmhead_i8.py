@@ -145,6 +145,8 @@ def operands(V, n, B, seed):
     return w, sw, xq, sx
 
 
+# a batch of each class of the tile rule, above and below five rows
+I8_TILE_BATCHES = [1, 9, 30, 60, 100, 200, 300]
 BATCHES = [1, 2, 3, 15, 16, 17, 32, 33, 64, 65, 100, 128, 129, 256, 257, 300]
 
 
@@ -181,6 +183,36 @@ def test_every_vocabulary(torch_cuda, V):
         run_product(torch_cuda, *operands(V, 160, B, V), label=(V, B))
 
 
+I8_TILE_VOCABS = [3000, 9000, 13000, 20000, 33000, 40000, 60000, 90000]
+
+
+@pytest.mark.parametrize("V", I8_TILE_VOCABS)
+def test_every_tile(torch_cuda, V):
+    """Each shape of pz_lmtile.h (test_lmhead_tiles.py shows that these reach
+    them all), at lengths that end inside a stage, whole sizes on the device."""
+    torch = torch_cuda
+    g = torch.Generator(device="cuda")
+    g.manual_seed(V)
+    for B in I8_TILE_BATCHES:
+        for n in (208, 400):
+            w = torch.randint(-128, 128, (V, n), generator=g, device="cuda", dtype=torch.int8)
+            xq = torch.randint(-128, 128, (B, n), generator=g, device="cuda", dtype=torch.int8)
+            sw = torch.rand(V, generator=g, device="cuda")
+            sx = torch.rand(B, generator=g, device="cuda")
+            y = torch.full((B, V), -7.0, device="cuda")
+            ids = torch.empty(B, dtype=torch.int32, device="cuda")
+            with pz.Sampler(B, 16) as s:
+                s.lm_head_i8(w, sw, V, n, xq, sx, B, n, y, V)
+                s.lm_head_argmax_i8(w, sw, V, n, xq, sx, B, n, ids)
+                s.sync()
+            acc = xq.float() @ w.float().t().contiguous()  # exact: 2^14 n < 2^24
+            exp = (acc * sw[None]) * sx[:, None]
+            assert torch.equal(y, exp), (V, B, n)
+            first = torch.where(exp == exp.amax(1, keepdim=True),
+                                torch.arange(V, device="cuda"), V).amin(1)
+            assert torch.equal(ids.long(), first), (V, B, n)
+
+
 def test_the_largest_sums(torch_cuda):
     """+-128 and +-127 throughout at the longest rows: the ends of int32, whose
     rounding to fp32 is part of the definition."""
@@ -209,11 +241,12 @@ def test_ties_nan_and_zero_scales(torch_cuda):
     run_product(torch_cuda, w, sw, xq, sx, label="channel scales")
 
 
-@pytest.mark.parametrize("B", [1, 32, 256])
-def test_the_workload_size(torch_cuda, B):
-    """128256 x 2560: quantised from fp32 on the device, product and ids."""
+@pytest.mark.parametrize("V,n", [(128256, 2560), (2100, 131056)])
+@pytest.mark.parametrize("B", [1, 9, 32, 60, 100, 256])
+def test_large_weights(torch_cuda, V, n, B):
+    """Weights past the Infinity Cache: quantised from fp32 on the device, product
+    and ids."""
     torch = torch_cuda
-    V, n = 128256, 2560
     g = torch.Generator(device="cuda")
     g.manual_seed(B)
     w = torch.randint(-127, 128, (V, n), generator=g, device="cuda", dtype=torch.int8)
@@ -232,8 +265,9 @@ def test_the_workload_size(torch_cuda, B):
     assert (xq.cpu().numpy() == q).all()
     same(sx.cpu().numpy(), sc)
     acc = torch.empty((B, V), dtype=torch.float64, device="cuda")
-    for r in range(0, V, 16384):
-        acc[:, r:r + 16384] = xq.double() @ w[r:r + 16384].double().t().contiguous()
+    step = (1 << 26) // n
+    for r in range(0, V, step):
+        acc[:, r:r + step] = xq.double() @ w[r:r + step].double().t().contiguous()
     exp = (acc.float() * sw[None]) * sx[:, None]
     assert torch.equal(y, exp)
     first = torch.where(exp == exp.amax(1, keepdim=True),
