@@ -467,6 +467,7 @@ typedef struct {
  * target forward over drafts; T = 1: decoding).  For head h of n_heads, with
  * key head h / (n_heads / n_kv_heads):
  *   out[b, t, h] = sum_p softmax_p(scale * q[b, t, h] . k[p]) v[p]
+ * with 0 < scale <= 2e38.
  * q row (b, t) at d_q + (b * T + t) * ld_q, n_heads x head_dim elements; out
  * alike with ld_out.  Sums and softmax in fp32; softmax weights are rounded
  * to the type before they meet the values, the result once more.  A node that

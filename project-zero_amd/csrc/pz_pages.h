@@ -21,10 +21,9 @@ PZ_HD int pz_pages_len(const PzPages& P, int len) {
   return len < 0 ? 0 : (len < most ? len : most);
 }
 
-// Slot of position p (0 <= p < max_blocks << shift) in *slot; false, and a slot
-// of page 0, where the table names no page.
-PZ_HD bool pz_pages_slot(const PzPages& P, const int32_t* table, int p, int64_t* slot) {
-  const int32_t page = table[p >> P.shift];
+// Slot of position p, whose table entry reads `page`, in *slot; false, and a slot
+// of page 0, where that is no page of the cache.
+PZ_HD bool pz_pages_slot(const PzPages& P, int32_t page, int p, int64_t* slot) {
   const bool ok = (uint32_t)page < (uint32_t)P.n_blocks;
   *slot = ((int64_t)(ok ? page : 0) << P.shift) + (p & ((1 << P.shift) - 1));
   return ok;

@@ -86,7 +86,9 @@ inline PzRefusal pz_refuse_tree(const pz_kv_cache* c, const void* d_kn, const vo
   if (r.code) return r;
   if (n_heads <= 0 || n_heads % c->n_kv_heads)
     return {PZ_EINVAL, "n_heads is a multiple of n_kv_heads"};
-  if (!(scale > 0.0f) || scale > 3.0e38f) return {PZ_EINVAL, "scale is positive and finite"};
+  // (the kernels take scale log2(e), which has to be finite, too)
+  if (!(scale > 0.0f) || scale > 2.0e38f)
+    return {PZ_EINVAL, "scale is positive, at most 2e38"};
   const long row = (long)n_heads * c->head_dim;
   if (!d_q || !d_out || ld_q < row || ld_out < row) return {PZ_EINVAL, "bad q or out"};
   if (ld_q % 8 || ld_out % 8 || !pz_aligned16(d_q) || !pz_aligned16(d_out))

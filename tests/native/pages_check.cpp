@@ -22,7 +22,7 @@ int main() {
       for (int i = 0; i < size; i++) {
         const int p = page * size + i;
         int64_t slot = -1;
-        const bool ok = pz_pages_slot(P, table, p, &slot);
+        const bool ok = pz_pages_slot(P, table[p >> shift], p, &slot);
         check(ok == (table[page] >= 0 && table[page] < 7), "validity", p);
         check(slot == (int64_t)(ok ? table[page] : 0) * size + i, "slot", p);
         check(slot >= 0 && slot < 7 * (int64_t)size, "a slot of the cache", p);
@@ -37,7 +37,7 @@ int main() {
   const int32_t far[1] = {INT_MAX - 1};
   const PzPages F = {INT_MAX, 6, 1};
   int64_t slot = 0;
-  check(pz_pages_slot(F, far, 63, &slot) && slot == (int64_t)(INT_MAX - 1) * 64 + 63, "far", 63);
+  check(pz_pages_slot(F, far[0], 63, &slot) && slot == (int64_t)(INT_MAX - 1) * 64 + 63, "far", 63);
   check(pz_pages_most(-1, 5) == 0 && pz_pages_most(0, 5) == 0 && pz_pages_most(4, 5) == 4 &&
             pz_pages_most(6, 5) == 5,
         "counts", 5);

@@ -156,6 +156,7 @@ int main() {
   tree("tree: three heads over two", PZ_EINVAL, C { N; a.heads = 3; });
   tree("tree: scale 0", PZ_EINVAL, C { N; a.scale = 0.0f; });
   tree("tree: scale NaN", PZ_EINVAL, C { N; a.scale = __builtin_nanf(""); });
+  tree("tree: scale times log2(e) infinite", PZ_EINVAL, C { N; a.scale = 2.9e38f; });
   tree("tree: scale infinite", PZ_EINVAL, C { N; a.scale = __builtin_inff(); });
   tree("tree: null q", PZ_EINVAL, C { N; a.q = nullptr; });
   tree("tree: null out", PZ_EINVAL, C { N; a.out = nullptr; });

@@ -262,6 +262,56 @@ def test_what_is_not_seen_has_no_influence(torch_cuda, sampler, kind):
                     assert torch.isfinite(o.cpu()[~at]).all(), (b, t)
 
 
+@pytest.mark.parametrize("kind,D", [("bf16", 64), ("bf16", 128), ("fp16", 128), ("fp16", 64)])
+@pytest.mark.parametrize("T", [6, 16, 17, 40, 64])
+def test_many_rows_in_splits(torch_cuda, sampler, kind, D, T):
+    """Sequences of several splits, of one and of none, tiles that end early and
+    pages that are missing in the middle, at a range's ends and throughout, for
+    rows that fill their waves and rows that do not."""
+    c = Case(torch_cuda, kind, [1500, 0, 31, 1000, 257], T, 16, 2, D, 16, 7 * T).random_tree(T)
+    c.n_nodes = [T, T - 1, T, 1, T // 2]
+    c.table[0, 20] = -1
+    c.table[0, 93] = c.n_pages
+    c.table[3, 0] = 2 ** 31 - 1
+    c.table[4, 16] = -5
+    c.run(sampler, (kind, D, T))
+    c.table[3, :] = -1
+    c.run(sampler, "a sequence without pages")
+
+
+def test_many_rows_of_long_tables(torch_cuda, sampler):
+    """Tables of more entries than a workgroup keeps at hand."""
+    c = Case(torch_cuda, "bf16", [300, 7] * 16, 9, 64, 8, 64, 8, 77)
+    small = c.per
+    c.per = 2300
+    table = torch_cuda.full((32, c.per), -1, dtype=torch_cuda.int32)
+    table[:, :small] = c.table
+    c.table = table
+    c.run(sampler)
+    c.lens[3] = 2 ** 31 - 1  # all of the table: entries of no page from the first ones on
+    c.run(sampler, "the whole table")
+
+
+def test_many_rows_of_far_slots(torch_cuda, sampler):
+    """Slots 128 MiB apart: a tile's rows pass 32 bits of offsets."""
+    torch = torch_cuda
+    c = Case(torch, "bf16", [13], 12, 8, 2, 64, 8, 78, spare=0)
+    d = c.device()
+    ld, pages = 1 << 26, c.per
+    pool = torch.empty(((pages * 8 - 1) * ld + 1024,), dtype=torch.bfloat16, device="cuda")
+    at = torch.arange(pages)
+    for name, first in (("k", 0), ("v", 512)):
+        rows = getattr(c, name)[c.slots(0, torch.arange(pages * 8))].cuda()
+        pool[first:].as_strided((pages * 8, 128), (ld, 1)).copy_(rows)
+    cache = pz.kv_cache(type=pz.PZ_BF16, n_kv_heads=2, head_dim=64, d_k=pool, d_v=pool[512:], ld=ld,
+                        n_blocks=pages, block_size=8, d_blocks=at.int().reshape(1, -1).cuda(),
+                        max_blocks=pages, d_len=d["lens"])
+    sampler.tree_attention(cache, d["kn"], d["vn"], 128, 1, 12, 8, c.scale, d["q"], 512, d["out"],
+                           512)
+    sampler.sync()
+    c.check(d["out"])
+
+
 def test_large_scores(torch_cuda, sampler):
     """Scores far apart: one key takes all the weight, wherever it lies."""
     for kind in KINDS:
