@@ -155,10 +155,11 @@ int quant(pz_sampler* s, const void* d_x, long ldx, int rows, int n, int8_t* d_q
 //   * WK > 1 for few rows of W, whose waves would be too few to cover the loads'
 //     latency: 128 batch rows at 1292 x 6832 51 us with 256-row tiles, 16 so.
 //   * The shape: pz_lmtile.h (i8_tile_for).  128256 x 2560: batch 1 50 us (6.6
-//     TB/s), 16 58, 32 61, 64 67, 128 88, 256 117-125; bound by one read of W to
-//     64 batch rows, then by the stages (fragment reads and products of 256 x 256
-//     tiles: 1.7 us of 64 KiB each) and the logits' 131 MB, which a workgroup
-//     writes between its tiles.  32 x 32 x 32 products take as long (109 us fused
+//     TB/s), 16 58, 32 61, 64 67, 128 87, 256 111-118; bound by one read of W to
+//     64 batch rows, then by LDS (a stage of a 256 x 256 tile: 192 KiB of fragments
+//     and 64 KiB of loads are 0.99 us of it, its products 0.97; 2.2 us in all) and
+//     the logits' 131 MB, which a workgroup writes between its tiles (89 us without
+//     them, 67 without loads either).  32 x 32 x 32 products take as long (109 us fused
 //     at 256; 16 x 16 x 64 104) and write the logits in 32-byte pieces.
 //   * Workgroups start k at different stages, so that rows a multiple of 4 KiB
 //     apart do not all meet in the same memory channels.
@@ -426,6 +427,58 @@ __global__ __launch_bounds__(64 * WR * WC * WK) void k_lmhead_i8(
     const int b = b0 + (wc * TC + j) * 16 + m;
     fx[j] = b < nb ? sx[b] : 0.0f;
   }
+  const bool vec = MODE == 0 && (ld & 3) == 0 && ((uintptr_t)logits & 15) == 0;
+  // A tile's logits go out as whole rows of the batch, 256 bytes and more together:
+  // the workgroup turns 16 batch rows of each wc at a time in LDS.  (256 x 2560 x
+  // 128256 131 -> 123 us, to 50257 logits, whose rows are off 16 bytes, 74 -> 64; a
+  // batch of 8 the same.  Written past the caches they take 114, but then what reads
+  // them next loses more: with their maxima 148 -> 154.)
+  constexpr int RS = ROWS + 4, CG = WC * 16;  // floats of a row there, rows
+  constexpr bool TURN = MODE == 0 && WK == 1 && ROWS >= 64 && SH >= CG * RS * 4;
+  if constexpr (TURN) {
+    constexpr int NB = SH >= 2 * CG * RS * 4 ? 2 : 1, TH = 64 * NW;
+    __syncthreads();  // the ring is free
+#pragma unroll
+    for (int j = 0; j < TC; j++) {
+      float* turn = reinterpret_cast<float*>(sh) + (j % NB) * CG * RS;
+      if (NB == 1 && j > 0) __syncthreads();
+#pragma unroll
+      for (int t = 0; t < TR; t++) {
+        const int r = (wr * TR + t) * 16 + 4 * g;
+        lm_f32x4 y;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          y[i] = ((float)acc[t][j][i] * (row0 + r + i < V ? sw[row0 + r + i] : 0.0f)) * fx[j];
+        *reinterpret_cast<lm_f32x4*>(turn + (wc * 16 + m) * RS + r) = y;
+      }
+      __syncthreads();
+      auto batch = [&](int c) { return b0 + ((c >> 4) * TC + j) * 16 + (c & 15); };
+      if (vec) {
+#pragma unroll 4
+        for (int i = tid; i < CG * ROWS / 4; i += TH) {
+          const int c = i / (ROWS / 4), r = i % (ROWS / 4) * 4, row = row0 + r, b = batch(c);
+          if (b >= nb) continue;
+          const lm_f32x4 y = *reinterpret_cast<const lm_f32x4*>(turn + c * RS + r);
+          float* o = logits + (size_t)b * ld + row;
+          if (row + 3 < V) {
+            *reinterpret_cast<lm_f32x4*>(o) = y;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              if (row + e < V) o[e] = y[e];
+          }
+        }
+      } else {
+#pragma unroll 4
+        for (int i = tid; i < CG * ROWS; i += TH) {
+          const int c = i / ROWS, r = i % ROWS, row = row0 + r, b = batch(c);
+          if (b >= nb || row >= V) continue;
+          logits[(size_t)b * ld + row] = turn[c * RS + r];
+        }
+      }
+    }
+    return;
+  }
   // (rows in descending order, so that >= leaves the first of equal ones, and
   // -infinity counts where there is nothing above it; NaN never does)
   float bv[TC];
@@ -435,7 +488,6 @@ __global__ __launch_bounds__(64 * WR * WC * WK) void k_lmhead_i8(
     bv[j] = -__builtin_inff();
     bi[j] = -1;
   }
-  const bool vec = MODE == 0 && (ld & 3) == 0 && ((uintptr_t)logits & 15) == 0;
 #pragma unroll
   for (int t = TR - 1; t >= 0; t--) {
       const int row = row0 + (wr * TR + t) * 16 + 4 * g;
