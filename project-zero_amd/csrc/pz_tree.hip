@@ -23,7 +23,7 @@
 //     2^(TH + OFF), and the cross-lane maximum and the rescaling drop out of
 //     most tiles.
 //
-// k_tree, up to 32 rows: a workgroup owns 16 RT rows of one key head of one
+// k_tree, up to 32 rows or little work: a workgroup owns 16 RT rows of one key head of one
 // sequence and a range of its keys; its waves take tiles in turn, each with its
 // own m, l and result, which meet in LDS at the end.  Keys and values go from
 // memory to registers, with no barrier on the way.  Bound by memory: 32 ragged
@@ -31,11 +31,13 @@
 // 73 us, 3.7 TB/s; 55 us (4.9 TB/s) where all are of 2048, since one workgroup a
 // CU waits for the longest.
 //
-// k_tree_wide, more rows: the waves of a workgroup own 16 RT rows each and share
+// k_tree_wide, many rows over many keys: the waves of a workgroup own 16 RT rows each and share
 // the keys, whose tiles come to LDS through a ring of loads.  Bound by issue: 8 x
-// 64 nodes over 32768 positions 366 us (275 GFLOP at 0.75 PFLOP/s, 2.9 TB/s of
-// keys and values): 257 with no loads and no barrier, 297 with the barrier, 341
-// without the LDS reads.
+// 64 nodes over 32768 positions 343 us (275 GFLOP at 0.80 PFLOP/s, 3.1 TB/s of
+// keys and values).  Of a tile's 1.3 us a SIMD's two waves take 0.5 for the
+// products, 0.6 for the other vector instructions, and LDS 0.55 for the fragments
+// and the loads; before the fragments were read a phase ahead it was 363 us, 257 of
+// it without loads and barriers.
 //
 // Few rows and long sequences: the keys are split over S workgroups, whose
 // results k_tree_join adds up.
@@ -63,7 +65,7 @@ typedef _Float16 tr_f16x2 __attribute__((ext_vector_type(2)));
 constexpr int TR_JOIN = 4;          // waves of a joining workgroup
 constexpr int TR_KEYS = 32;         // keys of a tile
 constexpr int TR_ENTRIES = 2048;    // table entries of a split of the wide kernel
-constexpr int TR_STAGES = 5;        // tiles of its ring (4: the same time within 1 %)
+constexpr int TR_STAGES = 6;        // tiles of its ring
 constexpr int TR_WIDE = 8;          // its waves
 constexpr float TR_LOW = -3.0e38f;  // m before any score (finite: m - m is 0)
 constexpr float TR_LOG2E = 1.44269504088896340736f;
@@ -203,12 +205,16 @@ struct TrRows {
 #pragma unroll
       for (int i = 0; i < NW; i++) vr[e][i] = on >> e & 1u ? vr[e][i] : 0u;
   }
-  // the largest score of each row tile in this lane
+  // the largest score of each row tile in this lane (a NaN stays: its row's result is
+  // one, and the plain maximum would first quiet every operand)
+  __device__ __forceinline__ static float most(float a, float b) {
+    return __builtin_elementwise_maximum(a, b);
+  }
   __device__ __forceinline__ static void tops(const tr_f32x4 (&s)[RT][2], float (&tm)[RT]) {
 #pragma unroll
     for (int rt = 0; rt < RT; rt++)
-      tm[rt] = fmaxf(fmaxf(fmaxf(s[rt][0][0], s[rt][0][1]), fmaxf(s[rt][0][2], s[rt][0][3])),
-                     fmaxf(fmaxf(s[rt][1][0], s[rt][1][1]), fmaxf(s[rt][1][2], s[rt][1][3])));
+      tm[rt] = most(most(most(s[rt][0][0], s[rt][0][1]), most(s[rt][0][2], s[rt][0][3])),
+                    most(most(s[rt][1][0], s[rt][1][1]), most(s[rt][1][2], s[rt][1][3])));
   }
   // raises m where a score passes it by far
   __device__ __forceinline__ void raise(const float (&tm)[RT]) {
@@ -592,7 +598,8 @@ k_tree(const TreeArgs A) {
 // whose tiles come straight to LDS through a ring of TR_STAGES -- whole rows of
 // keys and of values, one barrier per tile -- instead of to every wave's
 // registers.  Waves past the last row load only, which is worth having: 48 rows
-// in 8 waves 83 us, in 4 111 (32 ragged sequences of up to 4096 positions).  The
+// in 8 waves 83 us, in 4 111 (32 ragged sequences of up to 4096 positions; 78
+// since fragments are read a phase before their products).  The
 // 16-byte pieces of a key's row are permuted so that the 16 rows that one cycle
 // reads lie in 16 places.
 template <int TYPE, int D, int RT>
@@ -737,10 +744,10 @@ k_tree_wide(const TreeArgs A) {
   Rows R;
   R.clear(lane, A.c);
   int buf = 0, nbuf = NS - 1;
-  // Tiles tl and tl + 1 have arrived, in every wave; and every wave is done with the
+  // Tiles tl to tl + 2 have arrived, in every wave; and every wave is done with the
   // slot of the tile before, which is filled next.
   auto step = [&](int tl) {
-    lm_wait<(NS - 3) * PER>();
+    lm_wait<(NS - 4) * PER>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     issue(clip(tl + NS - 1), ids, nbuf);
@@ -760,37 +767,35 @@ k_tree_wide(const TreeArgs A) {
     R.scores([&](int t, int ks) { return kf(at, t, ks); },
              [&](int rt, int ks) { return qf[rt][ks]; });
   };
-  // words i0 .. i0 + N - 1 of each key's values
-  auto fetch_v = [&](int i0, auto& vr) {
-    const char* vt = sh + buf * STG + TILE;
-    constexpr int N = sizeof(vr[0]) / 4;
+  // the words of a key's values in this lane
+  auto fetch = [&](const char* p, uint32_t(&v)[NW]) {
+    if constexpr (NW == 2) {
+      const tr_u32x2 x = *reinterpret_cast<const tr_u32x2*>(p);
+      v[0] = x[0];
+      v[1] = x[1];
+    } else {
+      static_assert(NW == 4, "");
+      const tr_u32x4 x = *reinterpret_cast<const tr_u32x4*>(p);
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      const char* p = vt + (16 * (e >> 2) + 4 * g + (e & 3)) * D * 2 + m * NT * 2 + 4 * i0;
-      if constexpr (N == 2) {
-        const tr_u32x2 x = *reinterpret_cast<const tr_u32x2*>(p);
-        vr[e][0] = x[0];
-        vr[e][1] = x[1];
-      } else {
-        static_assert(N == 4, "");
-        const tr_u32x4 x = *reinterpret_cast<const tr_u32x4*>(p);
-#pragma unroll
-        for (int c = 0; c < 4; c++) vr[e][c] = x[c];
-      }
+      for (int i = 0; i < 4; i++) v[i] = x[i];
     }
   };
   int tl = tl0;
   const int tc = tl1 < nc ? tl1 : nc;  // the cache's tiles end here
-  lm_wait<(NS - 2) * PER>();
+  lm_wait<(NS - 3) * PER>();
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
+  constexpr int NQ = 2 * KS;  // fragments of a tile's keys
+  tr_u32x4 kr[NQ];            // those of tile tl + 1
   float tm[RT] = {};
   if (!idle && tl < tc) {
     scores(0);
     R.tops(R.s, tm);
+#pragma unroll
+    for (int q = 0; q < NQ; q++) kr[q] = kf(1, q & 1, q >> 1);
   }
-  // The weights and values of a tile beside the scores of the next: the products
-  // run while the exponentials and permutes issue.
+  // The weights of a tile beside the scores of the next, its values beside that
+  // one's keys, each fragment read a phase before its product.
 #pragma clang loop unroll(disable)
   for (; tl < tc; tl++) {
     step(tl);
@@ -810,43 +815,39 @@ k_tree_wide(const TreeArgs A) {
         R.tops(R.s, tm);
       }
       R.raise(tm);
-      const int after = buf + 1 == NS ? 0 : buf + 1;
+      const int ahead = buf + 2 >= NS ? buf + 2 - NS : buf + 2;
+      const char* vt = sh + buf * STG + TILE + 4 * g * D * 2 + m * NT * 2;
+      uint32_t vr[8][NW];
       tr_f32x4 sn[RT][2];  // (of whatever lies there after the last of them: unused)
 #pragma unroll
       for (int rt = 0; rt < RT; rt++)
 #pragma unroll
         for (int t = 0; t < 2; t++) sn[rt][t] = tr_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int ks = 0; ks < KS; ks++)
+      for (int q = 0; q < NQ; q++) {
+        constexpr int EQ = 8 / NQ;  // weights and keys' values beside each
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-          const tr_u32x4 a = kf(after, t, ks);
+        for (int rt = 0; rt < RT; rt++)
+          sn[rt][q & 1] = TrType<TYPE>::mfma(kr[q], qf[rt][q >> 1], sn[rt][q & 1]);
 #pragma unroll
-          for (int rt = 0; rt < RT; rt++) {
-            sn[rt][t] = TrType<TYPE>::mfma(a, qf[rt][ks], sn[rt][t]);
-            constexpr int EW = 8 / (2 * KS) > 0 ? 8 / (2 * KS) : 1;  // weights beside each
-            const int q = (ks * 2 + t) * EW;
+        for (int e = q * EQ; e < (q + 1) * EQ; e++) {
 #pragma unroll
-            for (int e = 0; e < EW; e++)
-              if (q + e < 8) R.weigh(rt, q + e);
-          }
-        }
-      tr_u32x4 pf[RT];
-      R.pack(pf);
-      R.tops(sn, tm);
-      constexpr int HV = NW > 2 ? 2 : 1, WH = NW / HV;
-#pragma unroll
-      for (int hv = 0; hv < HV; hv++) {
-        uint32_t vr[8][WH];
-        fetch_v(hv * WH, vr);
-#pragma unroll
-        for (int nt = 0; nt < 2 * WH; nt++) {
-          uint32_t v[8];
-#pragma unroll
-          for (int e = 0; e < 8; e++) v[e] = vr[e][nt >> 1];
-          R.value(hv * 2 * WH + nt, v, nt & 1, pf);
+          for (int rt = 0; rt < RT; rt++) R.weigh(rt, e);
+          fetch(vt + (16 * (e >> 2) + (e & 3)) * D * 2, vr[e]);
         }
       }
+      tr_u32x4 pf[RT];
+      R.pack(pf);
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) {
+        uint32_t v[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = vr[e][nt >> 1];
+        R.value(nt, v, nt & 1, pf);
+#pragma unroll
+        for (int q = nt * NQ / NT; q < (nt + 1) * NQ / NT; q++) kr[q] = kf(ahead, q & 1, q >> 1);
+      }
+      R.tops(sn, tm);
 #pragma unroll
       for (int rt = 0; rt < RT; rt++)
 #pragma unroll
@@ -868,7 +869,9 @@ k_tree_wide(const TreeArgs A) {
 #pragma unroll
       for (int rt = 0; rt < RT; rt++) of_tile[rt] = sees[rt] >> node0;
       scores(buf);
-      fetch_v(0, vr);
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        fetch(sh + buf * STG + TILE + (16 * (e >> 2) + 4 * g + (e & 3)) * D * 2 + m * NT * 2, vr[e]);
       R.drop(on, [&](int rt, int key) { return of_tile[rt] >> key & 1ull; });
       R.blank(on, vr);
       R.weights();
@@ -1071,13 +1074,19 @@ int run_rows(pz_sampler* s, TreeArgs& A) {
       if (tiles <= 24 && heads <= s->n_cu) return narrow<TYPE, D, 1, 8>(s, A, tiles, 1);
     return narrow<TYPE, D, 1, 4>(s, A, tiles, splits(heads));
   }
-  // Where waves have a SIMD each (64 rows in 16s, 128 in 32s) they take the fewer
-  // rows.  32 ragged sequences of up to 4096 positions, us narrow / wide of 16 rows
-  // a wave / of 32: 20 rows 73 / 81; 48 98 / 83 / 100; 64 - / 85 / 100; 96 - / 106 /
-  // 100; 128 - / 110 / 102; 256 - / 197 / 157.
+  // The wide kernel (us, narrow / wide of 16 rows a wave / of 32):
+  //   32 ragged sequences of up to 4096 positions x 8 key heads: 20 rows 73 / 74; 32
+  //   74 / 76; 48 97 / 78 / 90; 64 - / 78 / 90; 96 - / 95 / 90; 128 - / 105 / 91; 256 -
+  //   / 181 / 142: from 33 rows on, and 16 a wave while each has a SIMD.
+  //   256 rows, 8 sequences x 8 key heads, by positions: 500 22 / - / 38; 1000 31 / -
+  //   / 40; 2000 51 / - / 50; 4000 96 / - / 73; one sequence 2000 18 / - / 25, 8000 33
+  //   / - / 34, 16000 49 / - / 41; 48 rows 8000 16 / 17, 32768 41 / 36: from 16
+  //   tiles a CU on, below which k_tree's row blocks fill more CUs; but with a
+  //   workgroup for each CU at once (32 x 8) 100 47 / - / 35, 48 rows 250 17 / 15.
   if constexpr (D < 256) {
     // (its offsets within a load's rows are 32 bits)
-    if (rows > 32 && A.ld < (1 << 26) && A.ld_n < (1 << 24)) {
+    if (rows > 32 && (heads >= s->n_cu || heads * tiles >= 16 * s->n_cu) && A.ld < (1 << 26) &&
+        A.ld_n < (1 << 24)) {
       const int rc = rows <= 64
                          ? wide<TYPE, D, 1>(s, A, tiles, splits(heads))
                          : wide<TYPE, D, 2>(s, A, tiles, splits(heads * ((rows + 255) / 256)));

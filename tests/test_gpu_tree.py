@@ -229,12 +229,13 @@ def test_rows_that_see_nothing(torch_cuda, sampler):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "fp16"])
-def test_what_is_not_seen_has_no_influence(torch_cuda, sampler, kind):
+@pytest.mark.parametrize("spare", [2, 1400])
+def test_what_is_not_seen_has_no_influence(torch_cuda, sampler, kind, spare):
     """NaN and infinities in nodes that a row does not see leave it as it is;
     rows that see them get what the sum gives."""
     torch = torch_cuda
     for T, D in ((6, 64), (40, 128), (33, 256)):
-        c = Case(torch, kind, [70, 0, 33], T, 8, 2, D, 16, 41).random_tree(5)
+        c = Case(torch, kind, [70, 0, 33], T, 8, 2, D, 16, 41, spare=spare).random_tree(5)
         clean = c.run(sampler, "clean")
         c.vn[:, 2] = float("nan")
         c.vn[:, 3, ::3] = float("inf")
@@ -264,11 +265,14 @@ def test_what_is_not_seen_has_no_influence(torch_cuda, sampler, kind):
 
 @pytest.mark.parametrize("kind,D", [("bf16", 64), ("bf16", 128), ("fp16", 128), ("fp16", 64)])
 @pytest.mark.parametrize("T", [6, 16, 17, 40, 64])
-def test_many_rows_in_splits(torch_cuda, sampler, kind, D, T):
+@pytest.mark.parametrize("spare", [2, 900])
+def test_many_rows_in_splits(torch_cuda, sampler, kind, D, T, spare):
     """Sequences of several splits, of one and of none, tiles that end early and
     pages that are missing in the middle, at a range's ends and throughout, for
-    rows that fill their waves and rows that do not."""
-    c = Case(torch_cuda, kind, [1500, 0, 31, 1000, 257], T, 16, 2, D, 16, 7 * T).random_tree(T)
+    rows that fill their waves and rows that do not, in tables that are short
+    and long."""
+    c = Case(torch_cuda, kind, [1500, 0, 31, 1000, 257], T, 16, 2, D, 16, 7 * T,
+             spare=spare).random_tree(T)
     c.n_nodes = [T, T - 1, T, 1, T // 2]
     c.table[0, 20] = -1
     c.table[0, 93] = c.n_pages
