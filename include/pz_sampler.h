@@ -440,9 +440,10 @@ PZ_API int pz_lm_head_argmax_i8(pz_sampler *s, const int8_t *d_w, const float *d
  * x head_dim keys start at d_k + i * ld elements, its values at d_v + i * ld.
  * d_len [B]: positions that hold committed tokens (clamped to [0, max_blocks *
  * block_size]).  block_size: a power of two, at least 8.  type: PZ_BF16 or
- * PZ_F16.  head_dim: 64, 128 or 256.  ld a multiple of 8, d_k and d_v 16-byte
- * aligned.  A page number outside [0, n_blocks) holds no positions: reading
- * leaves them out, as if they were masked, and writing skips them. */
+ * PZ_F16.  head_dim: 64, 128 or 256.  n_kv_heads (and n_heads of the calls):
+ * up to 65536.  ld a multiple of 8, d_k and d_v 16-byte aligned.  A page
+ * number outside [0, n_blocks) holds no positions: reading leaves them out, as
+ * if they were masked, and writing skips them. */
 typedef struct {
   int type;
   int n_kv_heads;

@@ -12,7 +12,11 @@ struct PzRefusal {
   const char* why;  // nullptr then
 };
 constexpr int PZ_MOST = 1 << 30;  // of ids and list entries, so that 32-bit counters can step past
+constexpr int PZ_MOST_HEADS = 1 << 16;  // so that rows and row lengths fit 32 bits
 constexpr PzRefusal PZ_TAKEN = {PZ_OK, nullptr};
+
+// Whether a launch of `wgs` workgroups fits: their threads have 32-bit numbers.
+inline bool pz_launch_fits(int64_t wgs, int threads) { return wgs <= UINT32_MAX / threads; }
 
 inline bool pz_aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
@@ -43,6 +47,7 @@ inline PzRefusal pz_refuse_quant(const void* d_x, int x_type, long ldx, int rows
     return {PZ_EINVAL, "x_type is PZ_F32, PZ_BF16 or PZ_F16"};
   if (((uintptr_t)d_x & (x_type == PZ_F32 ? 3 : 1)) != 0)
     return {PZ_EINVAL, "d_x is not aligned to its type"};
+  if (!pz_launch_fits(rows, 256)) return {PZ_ERANGE, "more rows than a launch takes"};
   return PZ_TAKEN;
 }
 
@@ -69,6 +74,9 @@ inline PzRefusal pz_refuse_cache(const pz_kv_cache* c, const void* d_kn, const v
     return {PZ_EINVAL, "bad cache"};
   if (c->block_size < 8 || (c->block_size & (c->block_size - 1)) != 0)
     return {PZ_EINVAL, "block_size is a power of two, at least 8"};
+  if (c->n_kv_heads > PZ_MOST_HEADS) return {PZ_ERANGE, "n_kv_heads above 65536"};
+  if (!pz_launch_fits((int64_t)B * T, 256))
+    return {PZ_ERANGE, "more sequences and nodes than a launch takes"};
   if ((int64_t)c->max_blocks * c->block_size > INT32_MAX - 64)
     return {PZ_ERANGE, "max_blocks * block_size does not fit 32 bits"};
   const long row = (long)c->n_kv_heads * c->head_dim;
@@ -86,6 +94,7 @@ inline PzRefusal pz_refuse_tree(const pz_kv_cache* c, const void* d_kn, const vo
   if (r.code) return r;
   if (n_heads <= 0 || n_heads % c->n_kv_heads)
     return {PZ_EINVAL, "n_heads is a multiple of n_kv_heads"};
+  if (n_heads > PZ_MOST_HEADS) return {PZ_ERANGE, "n_heads above 65536"};
   // (the kernels take scale log2(e), which has to be finite, too)
   if (!(scale > 0.0f) || scale > 2.0e38f)
     return {PZ_EINVAL, "scale is positive, at most 2e38"};

@@ -321,7 +321,7 @@ int launch(pz_sampler* s, RulesArgs& A, int B, size_t slot_bytes) {
   A.S = (A.V + A.W - 1) / A.W;
   if (DENSE) A.cap = A.W;
   const int64_t grid = (int64_t)B * (A.S + A.count);
-  if (grid > INT32_MAX) return fail(s, PZ_ERANGE, "B=%d rows of V=%d", B, A.V);
+  if (!pz_launch_fits(grid, BLOCK)) return fail(s, PZ_ERANGE, "B=%d rows of V=%d", B, A.V);
   const size_t lds = (size_t)A.cap * slot_bytes + (DENSE ? 0 : (size_t)A.r.n_bias * 4);
   // (the counting workgroups and the mask words have LDS of their own)
   auto k = k_rules<DENSE, NQ, BLOCK>;

@@ -1008,7 +1008,8 @@ int plan(pz_sampler* s, TreeArgs& A, int64_t units, int64_t tiles, int64_t want)
   A.S = (int)((tiles + A.chunk - 1) / A.chunk);
   A.part = static_cast<float*>(s->tree_dev);
   A.ml = A.part + (size_t)units * A.S * ROWS * D;
-  if (units * RT * (D / 16) > INT32_MAX || (int64_t)A.B * A.n_kv * A.S * A.nblk > INT32_MAX / 2)
+  if (!pz_launch_fits(((int64_t)A.B * A.n_kv * A.S + 7) * A.nblk, 512) ||
+      !pz_launch_fits(units * RT * (D / 16), A.S > 1 ? 64 * TR_JOIN : 1))
     return fail(s, PZ_ERANGE, "B=%d sequences of T=%d nodes", A.B, A.T);
   return PZ_OK;
 }
@@ -1183,7 +1184,6 @@ extern "C" int pz_cache_append(pz_sampler* s, const pz_kv_cache* cache, const vo
   if (!s) return PZ_EINVAL;
   const PzRefusal no = pz_refuse_cache(cache, d_kn, d_vn, ld_n, B, T);
   if (no.code) return fail(s, no.code, "%s", no.why);
-  if ((int64_t)B * T > INT32_MAX) return fail(s, PZ_ERANGE, "B=%d sequences of T=%d nodes", B, T);
   if (B == 0) return PZ_OK;
   PZ_HIP(s, hipSetDevice(s->device));
   const TreeArgs A = args_of(cache, d_kn, d_vn, ld_n, B, T);

@@ -377,7 +377,7 @@ class Sampler:
     def rules(self, d_in, d_out, B, V, ld_in, ld_out, rules):
         """Penalties, biases and masks of logit_rules(...) applied to B rows,
         in place when d_out is d_in (asynchronous)."""
-        _sync_torch(d_in, d_out)
+        _sync_torch(d_in, d_out, *getattr(rules, "buffers", ()))
         self._check(self.lib.pz_rules_batch(self.h, _ptr(d_in), ld_in, _ptr(d_out), ld_out, B, V,
                                             ctypes.byref(rules)))
 
@@ -390,7 +390,7 @@ class Sampler:
     def lm_head_i8(self, d_w, d_sw, V, n, d_x, d_sx, B, ldx, d_logits, ld):
         """logits[b, i] = (W[i, :] . x[b, :]) * sw[i] * sx[b], int8 operands
         (asynchronous)."""
-        _sync_torch(d_w, d_x, d_logits)
+        _sync_torch(d_w, d_x, d_logits, d_sw, d_sx)
         self._check(self.lib.pz_lm_head_i8(self.h, _ptr(d_w), _ptr(d_sw), V, n, _ptr(d_x),
                                            _ptr(d_sx), B, ldx, _ptr(d_logits), ld))
 
@@ -404,14 +404,14 @@ class Sampler:
                        ld_out, d_n_nodes=None, d_tree=None):
         """Attention of T nodes per sequence over kv_cache(...) and along the
         tree, d_tree None: a chain (asynchronous)."""
-        _sync_torch(d_q, d_kn, d_out)
+        _sync_torch(d_q, d_kn, d_out, *getattr(cache, "buffers", ()))
         self._check(self.lib.pz_tree_attention(
             self.h, ctypes.byref(cache), _ptr(d_kn), _ptr(d_vn), ld_n, B, T, _ptr(d_n_nodes),
             _ptr(d_tree), n_heads, scale, _ptr(d_q), ld_q, _ptr(d_out), ld_out))
 
     def cache_append(self, cache, d_kn, d_vn, ld_n, B, T, d_take=None, d_count=None):
         """Accepted nodes' keys and values into the cache's pages (asynchronous)."""
-        _sync_torch(d_kn, d_vn)
+        _sync_torch(d_kn, d_vn, *getattr(cache, "buffers", ()))
         self._check(self.lib.pz_cache_append(self.h, ctypes.byref(cache), _ptr(d_kn), _ptr(d_vn),
                                              ld_n, B, T, _ptr(d_take), _ptr(d_count)))
 

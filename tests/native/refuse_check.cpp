@@ -62,6 +62,8 @@ int main() {
   expect("quant: no rows", pz_refuse_quant(f, PZ_F32, 8, 0, 8, i8, 8, f), PZ_OK);
   expect("quant: null x", pz_refuse_quant(nullptr, PZ_F32, 8, 2, 8, i8, 8, f), PZ_EINVAL);
   expect("quant: null q", pz_refuse_quant(f, PZ_F32, 8, 2, 8, nullptr, 8, f), PZ_EINVAL);
+  expect("quant: more rows than a launch", pz_refuse_quant(f, PZ_F32, 8, 1 << 24, 8, i8, 8, f),
+         PZ_ERANGE);
   expect("quant: null scale", pz_refuse_quant(f, PZ_F32, 8, 2, 8, i8, 8, nullptr), PZ_EINVAL);
   expect("quant: negative rows", pz_refuse_quant(f, PZ_F32, 8, -2, 8, i8, 8, f), PZ_EINVAL);
   expect("quant: empty rows", pz_refuse_quant(f, PZ_F32, 8, 2, 0, i8, 8, f), PZ_EINVAL);
@@ -154,6 +156,10 @@ int main() {
   tree("tree: v off 16 bytes", PZ_EINVAL, C { N; c.d_v = h + 4; });
   tree("tree: no heads", PZ_EINVAL, C { N; a.heads = 0; });
   tree("tree: three heads over two", PZ_EINVAL, C { N; a.heads = 3; });
+  tree("tree: more heads", PZ_ERANGE, C { N; a.heads = (1 << 16) + 2; a.ld_q = a.ld_out = 1L << 23; });
+  tree("tree: more key heads", PZ_ERANGE,
+       C { N; c.n_kv_heads = (1 << 16) + 2; a.heads = c.n_kv_heads; c.ld = a.ld_n = a.ld_q = a.ld_out = 1L << 23; });
+  tree("tree: more sequences than a launch", PZ_ERANGE, C { N; a.B = 1 << 23; });
   tree("tree: scale 0", PZ_EINVAL, C { N; a.scale = 0.0f; });
   tree("tree: scale NaN", PZ_EINVAL, C { N; a.scale = __builtin_nanf(""); });
   tree("tree: scale times log2(e) infinite", PZ_EINVAL, C { N; a.scale = 2.9e38f; });
@@ -164,6 +170,11 @@ int main() {
   tree("tree: out rows off 16 bytes", PZ_EINVAL, C { N; a.ld_out = 260; });
   tree("tree: q off 16 bytes", PZ_EINVAL, C { N; a.q = h + 2; });
   expect("tree: null cache", pz_refuse_cache(nullptr, h, h, 128, 2, 3), PZ_EINVAL);
+  expect("append: as many as a launch", pz_refuse_cache(&c0, h, h, 128, (1 << 18) - 1, 64), PZ_OK);
+  expect("append: more", pz_refuse_cache(&c0, h, h, 128, 1 << 18, 64), PZ_ERANGE);
+  expect("launch: all its threads", pz_launch_fits((1 << 24) - 1, 256) ? PZ_TAKEN : PzRefusal{PZ_ERANGE, ""}, PZ_OK);
+  expect("launch: one too many",
+         pz_launch_fits(1 << 24, 256) ? PZ_TAKEN : PzRefusal{PZ_ERANGE, ""}, PZ_ERANGE);
   expect("append: good", pz_refuse_cache(&c0, h, h, 128, 2, 3), PZ_OK);
   return bad != 0;
 }
