@@ -918,16 +918,20 @@ k_tree_wide(const TreeArgs A) {
   }
 }
 
-// Adds up the splits of one unit (key head and row block): a workgroup for each
-// float4 of a lane's results, its waves taking the splits in turn.
-template <int TYPE, int D, int RT>
+// Adds up the splits of one unit (key head and row block): for each float4 of a
+// lane's results WAVES waves, which take the splits in turn; TR_JOIN / WAVES of
+// them in a workgroup.  (One wave where the splits are few enough to be under way
+// together: 512 units of 4 splits of 32 rows 20
+// -> 11 us.)
+template <int TYPE, int D, int RT, int WAVES>
 __global__ __launch_bounds__(64 * TR_JOIN) void k_tree_join(const TreeArgs A) {
-  constexpr int NT = D / 16, ROWS = 16 * RT, CH = RT * NT;
-  __shared__ tr_f32x4 sum[TR_JOIN][64];
-  __shared__ float mls[TR_JOIN][16][2];
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int m = lane & 15, g = lane >> 4;
-  const int unit = blockIdx.x / CH, ch = blockIdx.x - unit * CH;
+  constexpr int NT = D / 16, ROWS = 16 * RT, CH = RT * NT, PER = TR_JOIN / WAVES;
+  static_assert(CH % PER == 0 && (WAVES == 1 || PER == 1), "a workgroup's work is one unit's");
+  __shared__ tr_f32x4 sum[WAVES][64];
+  __shared__ float mls[WAVES][16][2];
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int m = lane & 15, g = lane >> 4, w = wv % WAVES, at = blockIdx.x * PER + wv / WAVES;
+  const int unit = at / CH, ch = at - unit * CH;
   const int blk = unit % A.nblk, bh = unit / A.nblk, h = bh % A.n_kv, b = bh / A.n_kv;
   const int nn = tr_nodes(A, b), rows = nn * A.group;
   if (blk * ROWS >= rows) return;  // (its workgroups wrote nothing)
@@ -942,14 +946,14 @@ __global__ __launch_bounds__(64 * TR_JOIN) void k_tree_join(const TreeArgs A) {
   constexpr int U = 4;  // splits of a wave whose results are on their way together
   float mt = TR_LOW, lt = 0.0f;
   tr_f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s0 = w; s0 < ns; s0 += TR_JOIN * U) {
+  for (int s0 = w; s0 < ns; s0 += WAVES * U) {
     float ms[U], ls[U];
     tr_f32x4 v[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const int s = s0 + u * TR_JOIN < ns ? s0 + u * TR_JOIN : s0;  // (past the last: the first,
+      const int s = s0 + u * WAVES < ns ? s0 + u * WAVES : s0;  // (past the last: the first,
       ms[u] = ml[(size_t)s * ROWS * 2];                             // for nothing)
-      ls[u] = s0 + u * TR_JOIN < ns ? ml[(size_t)s * ROWS * 2 + 1] : 0.0f;
+      ls[u] = s0 + u * WAVES < ns ? ml[(size_t)s * ROWS * 2 + 1] : 0.0f;
       v[u] = part[(size_t)s * CH * 64];
     }
     float mn = mt;
@@ -963,29 +967,32 @@ __global__ __launch_bounds__(64 * TR_JOIN) void k_tree_join(const TreeArgs A) {
     for (int u = 0; u < U; u++) {
       const float e = __builtin_amdgcn_exp2f(ms[u] - mt);
       lt += ls[u] * e;
-      if (s0 + u * TR_JOIN < ns) o += v[u] * e;
+      if (s0 + u * WAVES < ns) o += v[u] * e;
     }
   }
-  sum[w][lane] = o;
-  if (g == 0) {
-    mls[w][m][0] = mt;
-    mls[w][m][1] = lt;
-  }
-  __syncthreads();
   const int r = blk * ROWS + rt * 16 + m;
-  if (w != 0 || r >= rows) return;
-  float mx = mt;
+  if constexpr (WAVES > 1) {
+    sum[w][lane] = o;
+    if (g == 0) {
+      mls[w][m][0] = mt;
+      mls[w][m][1] = lt;
+    }
+    __syncthreads();
+    if (w != 0) return;
+    float mx = mt;
 #pragma unroll
-  for (int k = 1; k < TR_JOIN; k++) mx = fmaxf(mx, mls[k][m][0]);
-  const float a0 = __builtin_amdgcn_exp2f(mt - mx);
-  lt *= a0;
-  o *= a0;
+    for (int k = 1; k < WAVES; k++) mx = fmaxf(mx, mls[k][m][0]);
+    const float a0 = __builtin_amdgcn_exp2f(mt - mx);
+    lt *= a0;
+    o *= a0;
 #pragma unroll
-  for (int k = 1; k < TR_JOIN; k++) {
-    const float e = __builtin_amdgcn_exp2f(mls[k][m][0] - mx);
-    lt += mls[k][m][1] * e;
-    o += sum[k][lane] * e;
+    for (int k = 1; k < WAVES; k++) {
+      const float e = __builtin_amdgcn_exp2f(mls[k][m][0] - mx);
+      lt += mls[k][m][1] * e;
+      o += sum[k][lane] * e;
+    }
   }
+  if (r >= rows) return;
   const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
   const int t = r / A.group, hq = h * A.group + (r - t * A.group);
   tr_store4<TYPE>(A.out + ((size_t)b * A.T + t) * A.ld_out + (size_t)hq * D + 4 * NT * g + NT * i +
@@ -1018,8 +1025,13 @@ template <int TYPE, int D, int RT>
 int join(pz_sampler* s, const TreeArgs& A, int64_t units) {
   PZ_HIP(s, hipGetLastError());
   if (A.S > 1) {
-    hipLaunchKernelGGL((k_tree_join<TYPE, D, RT>), dim3((unsigned)(units * RT * (D / 16))),
-                       dim3(64 * TR_JOIN), 0, s->stream, A);
+    const unsigned parts = (unsigned)(units * RT * (D / 16));
+    if (A.S <= 4)
+      hipLaunchKernelGGL((k_tree_join<TYPE, D, RT, 1>), dim3(parts / TR_JOIN), dim3(64 * TR_JOIN),
+                         0, s->stream, A);
+    else
+      hipLaunchKernelGGL((k_tree_join<TYPE, D, RT, TR_JOIN>), dim3(parts), dim3(64 * TR_JOIN), 0,
+                         s->stream, A);
     PZ_HIP(s, hipGetLastError());
   }
   return PZ_OK;
