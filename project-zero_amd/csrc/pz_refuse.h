@@ -47,7 +47,7 @@ inline PzRefusal pz_refuse_quant(const void* d_x, int x_type, long ldx, int rows
     return {PZ_EINVAL, "x_type is PZ_F32, PZ_BF16 or PZ_F16"};
   if (((uintptr_t)d_x & (x_type == PZ_F32 ? 3 : 1)) != 0)
     return {PZ_EINVAL, "d_x is not aligned to its type"};
-  if (!pz_launch_fits(rows, 256)) return {PZ_ERANGE, "more rows than a launch takes"};
+  if (!pz_launch_fits(rows, n > 8192 ? 1024 : 256)) return {PZ_ERANGE, "more rows than a launch takes"};
   return PZ_TAKEN;
 }
 
