@@ -474,11 +474,12 @@ typedef struct {
  * to the type before they meet the values, the result once more.  A node that
  * attends nothing gets zeros; what a node does not attend has no influence,
  * NaN included; rows of nodes from n_b on are left as they are.  ld_q, ld_n
- * and ld_out multiples of 8, pointers 16-byte aligned.  The work is laid out
- * for sequences as long as their tables (max_blocks * block_size): a table
- * not much longer than the longest sequence is fastest.  Long sequences are
- * split over workgroups, in a workspace that the first call allocates (64 MiB,
- * kept until the sampler is destroyed).
+ * and ld_out multiples of 8, pointers 16-byte aligned.  The host sees the
+ * tables' length (max_blocks * block_size) and chooses a kernel by it; the
+ * kernel shares the work out by the longest sequence's, so tables may be kept
+ * larger than needed.  Long sequences are split over workgroups, in a
+ * workspace that the first call allocates (64 MiB, kept until the sampler is
+ * destroyed).
  * Asynchronous on the sampler's stream; after that first call it can be
  * captured into a HIP graph.  Calls of one sampler, replays included, must be
  * ordered (on one stream or by events): they share the workspace. */

@@ -64,6 +64,7 @@ typedef _Float16 tr_f16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int TR_JOIN = 4;          // waves of a joining workgroup
 constexpr int TR_KEYS = 32;         // keys of a tile
+constexpr int TR_SHARE = 8;         // tiles that are worth a workgroup
 constexpr int TR_ENTRIES = 2048;    // table entries of a split of the wide kernel
 constexpr int TR_STAGES = 6;        // tiles of its ring
 constexpr int TR_WIDE = 8;          // its waves
@@ -127,13 +128,48 @@ struct TreeArgs {
   uint16_t* out;
   long ld_out;
   int S, nblk;  // most splits of a sequence, row blocks of a key head
-  int chunk;    // tiles of a split
+  int chunk;    // tiles of a split of the longest table
   float* part;  // [unit][S] results (TR result order), then their m and l
   float* ml;
 };
 
 __device__ __forceinline__ int tr_nodes(const TreeArgs& A, int b) {
   return A.n_nodes ? pz_pages_most(A.n_nodes[b], A.T) : A.T;
+}
+
+__device__ __forceinline__ int tr_tiles(const TreeArgs& A, int b) {
+  return (pz_pages_len(A.pages, A.len[b]) + TR_KEYS - 1) / TR_KEYS +
+         (tr_nodes(A, b) + TR_KEYS - 1) / TR_KEYS;
+}
+
+// Tiles of a split: a share of the longest sequence's, which tables that are kept
+// larger do not change (A.chunk: the longest table's, the most that it can be).
+// (Tables of 32768 positions, us by the table / by the longest sequence: one token
+// over 2000 17.7 / 12.4, 8 sequences x 64 nodes over 4000 141 / 64; tight tables the
+// same within 0.5.)
+__device__ __forceinline__ int tr_chunk(const TreeArgs& A, int b, int lane) {
+  if (A.S == 1) return A.chunk;
+  int most;
+  if (A.B == 1) {
+    most = tr_tiles(A, b);
+  } else {
+    most = 0;
+    for (int i = lane; i < A.B; i += 64) {
+      const int n = tr_tiles(A, i);
+      most = n > most ? n : most;
+    }
+    // the wave's maximum in lane 63: within 16 lanes, then over them
+    auto step = [&](int o) { most = o > most ? o : most; };
+    step(__builtin_amdgcn_update_dpp(0, most, 0x111, 0xf, 0xf, true));  // lane - 1
+    step(__builtin_amdgcn_update_dpp(0, most, 0x112, 0xf, 0xf, true));  // lane - 2
+    step(__builtin_amdgcn_update_dpp(0, most, 0x114, 0xf, 0xf, true));  // lane - 4
+    step(__builtin_amdgcn_update_dpp(0, most, 0x118, 0xf, 0xf, true));  // lane - 8
+    step(__builtin_amdgcn_update_dpp(0, most, 0x142, 0xa, 0xf, true));  // row 0's and 2's last to 1, 3
+    step(__builtin_amdgcn_update_dpp(0, most, 0x143, 0xc, 0xf, true));  // lane 31 to rows 2, 3
+    most = __builtin_amdgcn_readlane(most, 63);
+  }
+  const int share = (most + A.S - 1) / A.S;
+  return share < TR_SHARE ? TR_SHARE : share;
 }
 
 // A lane's results of one row: d = NT (4 g + i) + 4 f + 0..3 in o (i, f).
@@ -358,9 +394,10 @@ k_tree(const TreeArgs A) {
   const int rows = nn * A.group, row0 = blk * ROWS;
   if (row0 >= rows) return;
   const int nc = (ctx + TR_KEYS - 1) / TR_KEYS, ntl = nc + (nn + TR_KEYS - 1) / TR_KEYS;
-  const int tl0 = sp * A.chunk, tl1 = ntl - tl0 < A.chunk ? ntl : tl0 + A.chunk;
+  const int chunk = tr_chunk(A, b, lane);
+  const int tl0 = sp * chunk, tl1 = ntl - tl0 < chunk ? ntl : tl0 + chunk;
   if (tl0 >= ntl) return;
-  const int ns = (ntl + A.chunk - 1) / A.chunk;  // splits that this sequence has
+  const int ns = (ntl + chunk - 1) / chunk;  // splits that this sequence has
   const int32_t* table = A.blocks + (size_t)b * A.pages.max_blocks;
   const uint16_t* kc = A.k + (size_t)h * D;
   const uint16_t* vc = A.v + (size_t)h * D;
@@ -630,9 +667,10 @@ k_tree_wide(const TreeArgs A) {
   const int rows = nn * A.group, row0 = (wg * WAVES + w) * ROWS;
   if (wg * WAVES * ROWS >= rows) return;
   const int nc = (ctx + TR_KEYS - 1) / TR_KEYS, ntl = nc + (nn + TR_KEYS - 1) / TR_KEYS;
-  const int tl0 = sp * A.chunk, tl1 = ntl - tl0 < A.chunk ? ntl : tl0 + A.chunk;
+  const int chunk = tr_chunk(A, b, lane);
+  const int tl0 = sp * chunk, tl1 = ntl - tl0 < chunk ? ntl : tl0 + chunk;
   if (tl0 >= ntl) return;
-  const int ns = (ntl + A.chunk - 1) / A.chunk;  // splits that this sequence has
+  const int ns = (ntl + chunk - 1) / chunk;  // splits that this sequence has
   const bool idle = row0 >= rows;                // (a wave past the last row loads only)
   const uint16_t* kc = A.k + (size_t)h * D;
   const uint16_t* vc = A.v + (size_t)h * D;
@@ -935,9 +973,7 @@ __global__ __launch_bounds__(64 * TR_JOIN) void k_tree_join(const TreeArgs A) {
   const int blk = unit % A.nblk, bh = unit / A.nblk, h = bh % A.n_kv, b = bh / A.n_kv;
   const int nn = tr_nodes(A, b), rows = nn * A.group;
   if (blk * ROWS >= rows) return;  // (its workgroups wrote nothing)
-  const int ntl = (pz_pages_len(A.pages, A.len[b]) + TR_KEYS - 1) / TR_KEYS +
-                  (nn + TR_KEYS - 1) / TR_KEYS;
-  const int ns = (ntl + A.chunk - 1) / A.chunk;
+  const int chunk = tr_chunk(A, b, lane), ns = (tr_tiles(A, b) + chunk - 1) / chunk;
   if (ns <= 1) return;  // (its workgroup wrote the results)
   const int rt = ch / NT, i = ch % NT / (NT / 4), f = ch % (NT / 4);
   const float* ml = A.ml + ((size_t)unit * A.S * ROWS + rt * 16 + m) * 2;
@@ -1075,7 +1111,7 @@ int run_rows(pz_sampler* s, TreeArgs& A) {
   // its traffic: 32 x 5 nodes, 256 key heads, over 2048 positions whole 55 us, in
   // two splits 67.)
   auto splits = [&](int64_t wgs) {
-    const int64_t want = (s->n_cu + wgs - 1) / wgs, most = tiles / 8;
+    const int64_t want = (s->n_cu + wgs - 1) / wgs, most = tiles / TR_SHARE;
     return want < most ? want : most;
   };
   if (rows <= 16) {
