@@ -65,7 +65,7 @@ typedef _Float16 tr_f16x2 __attribute__((ext_vector_type(2)));
 constexpr int TR_JOIN = 4;          // waves of a joining workgroup
 constexpr int TR_KEYS = 32;         // keys of a tile
 constexpr int TR_SHARE = 8;         // tiles that are worth a workgroup
-constexpr int TR_ENTRIES = 2048;    // table entries of a split of the wide kernel
+constexpr int TR_ENTRIES = 2048;    // table entries that the wide kernel keeps in LDS
 constexpr int TR_STAGES = 6;        // tiles of its ring
 constexpr int TR_WIDE = 8;          // its waves
 constexpr float TR_LOW = -3.0e38f;  // m before any score (finite: m - m is 0)
@@ -706,7 +706,7 @@ k_tree_wide(const TreeArgs A) {
     if (tl0 < nc)
       for (int e = e0 + tid; e <= e1; e += 64 * WAVES) {
         const int32_t id = A.blocks[(size_t)b * A.pages.max_blocks + e];
-        tab[e - e0] = id;
+        if (e - e0 < TR_ENTRIES) tab[e - e0] = id;
         whole = whole && (uint32_t)id < (uint32_t)A.pages.n_blocks;
       }
     if (tid == 0) broken = 0;
@@ -715,7 +715,19 @@ k_tree_wide(const TreeArgs A) {
     __syncthreads();
     whole = broken == 0;
   }
-  auto entry = [&](int p) { return tab[(p >> A.pages.shift) - e0]; };
+  // (Entries past those that LDS holds: with a wait of their own, which is one for the
+  // ring's loads, too.)
+  auto entry = [&](int p) {
+    const int e = p >> A.pages.shift;
+    int32_t id;
+    if (e - e0 < TR_ENTRIES) {
+      id = tab[e - e0];
+    } else {
+      id = A.blocks[(size_t)b * A.pages.max_blocks + e];
+      __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    }
+    return id;
+  };
   struct Ids {
     int32_t v[PK];
   };
@@ -1085,8 +1097,6 @@ int narrow(pz_sampler* s, TreeArgs& A, int64_t tiles, int64_t want) {
   return join<TYPE, D, RT>(s, A, units);
 }
 
-// (PZ_ENOTSUP, without a message: a split has more table entries than the kernel
-// holds)
 template <int TYPE, int D, int RT>
 int wide(pz_sampler* s, TreeArgs& A, int64_t tiles, int64_t want) {
   const int nwg = (A.T * A.group + 16 * RT * TR_WIDE - 1) / (16 * RT * TR_WIDE);
@@ -1094,7 +1104,6 @@ int wide(pz_sampler* s, TreeArgs& A, int64_t tiles, int64_t want) {
   const int64_t units = (int64_t)A.B * A.n_kv * A.nblk;
   const int rc = plan<D, RT>(s, A, units, tiles, want);
   if (rc != PZ_OK) return rc;
-  if (((int64_t)A.chunk * TR_KEYS >> A.pages.shift) + 2 > TR_ENTRIES) return PZ_ENOTSUP;
   const int64_t groups = ((int64_t)A.B * A.n_kv * A.S + 7) / 8 * 8;
   hipLaunchKernelGGL((k_tree_wide<TYPE, D, RT>), dim3((unsigned)(groups * nwg)),
                      dim3(64 * TR_WIDE), 0, s->stream, A);
@@ -1135,12 +1144,9 @@ int run_rows(pz_sampler* s, TreeArgs& A) {
   if constexpr (D < 256) {
     // (its offsets within a load's rows are 32 bits)
     if (rows > 32 && (heads >= s->n_cu || heads * tiles >= 16 * s->n_cu) && A.ld < (1 << 26) &&
-        A.ld_n < (1 << 24)) {
-      const int rc = rows <= 64
-                         ? wide<TYPE, D, 1>(s, A, tiles, splits(heads))
-                         : wide<TYPE, D, 2>(s, A, tiles, splits(heads * ((rows + 255) / 256)));
-      if (rc != PZ_ENOTSUP) return rc;
-    }
+        A.ld_n < (1 << 24))
+      return rows <= 64 ? wide<TYPE, D, 1>(s, A, tiles, splits(heads))
+                        : wide<TYPE, D, 2>(s, A, tiles, splits(heads * ((rows + 255) / 256)));
   }
   return narrow<TYPE, D, 2, 4>(s, A, tiles, splits(heads * ((rows + 31) / 32)));
 }

@@ -287,13 +287,35 @@ def test_many_rows_of_long_tables(torch_cuda, sampler):
     """Tables of more entries than a workgroup keeps at hand."""
     c = Case(torch_cuda, "bf16", [300, 7] * 16, 9, 64, 8, 64, 8, 77)
     small = c.per
-    c.per = 2300
+    c.per = 4500
     table = torch_cuda.full((32, c.per), -1, dtype=torch_cuda.int32)
     table[:, :small] = c.table
     c.table = table
     c.run(sampler)
     c.lens[3] = 2 ** 31 - 1  # all of the table: entries of no page from the first ones on
     c.run(sampler, "the whole table")
+
+
+def test_many_sequences_of_long_tables(torch_cuda, sampler):
+    """As many entries in tables of many sequences."""
+    c = Case(torch_cuda, "bf16", [40, 7] * 32, 33, 32, 32, 64, 8, 79)
+    c.n_nodes = [0] * 64
+    c.n_nodes[5], c.n_nodes[62] = 33, 20
+    small = c.per
+    c.per = 4500
+    table = torch_cuda.full((64, c.per), -1, dtype=torch_cuda.int32)
+    table[:, :small] = c.table
+    c.table = table
+    c.run(sampler)
+
+
+def test_many_rows_of_a_long_sequence(torch_cuda, sampler):
+    """Positions whose table entries lie past those at hand, some without a page."""
+    c = Case(torch_cuda, "bf16", [16700, 7, 7, 7, 7, 7, 7, 40], 33, 32, 32, 64, 8, 80)
+    c.n_nodes = [2, 0, 0, 0, 0, 0, 0, 33]
+    c.table[0, 2050] = -1
+    c.table[0, 2087] = c.n_pages
+    c.run(sampler)
 
 
 def test_many_rows_of_far_slots(torch_cuda, sampler):
