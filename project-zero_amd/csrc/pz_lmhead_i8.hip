@@ -586,16 +586,19 @@ template <int MODE>
 int run(pz_sampler* s, const I8Call& c) {
   const bool fast = c.n % 16 == 0 && c.ldx % 16 == 0 && pz_aligned16(c.w) && pz_aligned16(c.x) &&
                     (int64_t)c.ldx * 256 <= UINT32_MAX;
-  const int tile = i8_tile_for(c.V, c.B, s->n_cu);
   if (!fast) {
-    // few rows of W: waves that share k, as above
-    if (tile == 0) return launch<1, 1, 4, 1, 1, 2, 2, MODE, false>(s, c);
-    if (c.B <= 16) return launch<4, 1, 1, 1, 1, 2, 2, MODE, false>(s, c);
-    if (tile == 3 || tile == 6) return launch<1, 1, 4, 1, 4, 2, 2, MODE, false>(s, c);
-    if (c.B <= 64) return launch<4, 1, 1, 2, 4, 2, 2, MODE, false>(s, c);
-    if (tile == 11 || tile == 15) return launch<1, 2, 4, 1, 4, 2, 2, MODE, false>(s, c);
-    return launch<4, 2, 1, 4, 4, 2, 2, MODE, false>(s, c);
+    switch (i8_odd_tile_for(c.V, c.B, s->n_cu)) {
+      case 0: return launch<2, 1, 4, 1, 1, 2, 2, MODE, false>(s, c);
+      case 1: return launch<2, 1, 2, 1, 1, 2, 2, MODE, false>(s, c);
+      case 2: return launch<2, 2, 2, 1, 2, 2, 2, MODE, false>(s, c);
+      case 3: return launch<2, 2, 1, 2, 2, 2, 2, MODE, false>(s, c);
+      case 4: return launch<4, 1, 1, 2, 4, 2, 2, MODE, false>(s, c);
+      case 5: return launch<2, 2, 2, 1, 4, 2, 2, MODE, false>(s, c);
+      case 6: return launch<2, 2, 2, 2, 4, 2, 2, MODE, false>(s, c);
+      default: return launch<4, 2, 1, 2, 4, 2, 2, MODE, false>(s, c);
+    }
   }
+  const int tile = i8_tile_for(c.V, c.B, s->n_cu);
   switch (tile) {
 #define PZ_I8_CASE(I, ...) \
   case I: return launch<__VA_ARGS__, MODE, true>(s, c)

@@ -76,15 +76,31 @@ constexpr I8Tile I8_TILE_SHAPES[] = {
     {256, 16, 24},  {256, 32, 40},  {256, 64, 70},  {256, 128, 140}, {256, 256, 0}}; // (15 - 19)
 constexpr int I8_TILE_COUNT = sizeof(I8_TILE_SHAPES) / sizeof(I8_TILE_SHAPES[0]);
 
+// The first shape of its batch rows that takes a W of V rows (cols: of a tile; more
+// batch rows are as many more workgroups).
+inline int i8_shape_for(const I8Tile* shapes, int count, int cols, int V, int B, int n_cu) {
+  const double rows = (double)V * ((B + cols - 1) / cols) / n_cu;
+  for (int i = 0; i < count; i++)
+    if (shapes[i].cols == cols && (shapes[i].most == 0 || rows <= shapes[i].most)) return i;
+  return count - 1;
+}
 inline int i8_tile_for(int V, int B, int n_cu) {
   const int cols = B <= 16 ? 16 : B <= 32 ? 32 : B <= 64 ? 64 : B <= 128 ? 128 : 256;
-  // (more than 256 batch rows: as many more workgroups)
-  const double rows = (double)V * ((B + cols - 1) / cols) / n_cu;
-  for (int i = 0; i < I8_TILE_COUNT; i++) {
-    const I8Tile& t = I8_TILE_SHAPES[i];
-    if (t.cols != cols) continue;
-    if (i == 1 && B <= 4) return i;
-    if (t.most == 0 || rows <= t.most) return i;
-  }
-  return I8_TILE_COUNT - 1;
+  const int i = i8_shape_for(I8_TILE_SHAPES, I8_TILE_COUNT, cols, V, B, n_cu);
+  return i == 2 && B <= 4 ? 1 : i;
+}
+
+// The same where rows are off 16 bytes and go through registers, at k = 2565: the
+// batch's rows cost as much as W's, so that tiles of more rows pay earlier.  8
+// batch rows 10000 14.6 / 15.5, 20000 19.4 / 17.9; 64 5000 18.3 / 25.2 / 32.9, 10000
+// 20.4 / 25.6, 20000 29.6 / 27.8 / 34.7, 60000 89 / 69 / 60; 200 2000 24.6 / 28.0, 5000
+// 33.6 / 28.0 / 35.2, 10000 49.5 / 49.9 / 35.9, 60000 - / 208 / 126 (256-row tiles
+// 124, but 5000 48.2).
+constexpr I8Tile I8_ODD_SHAPES[] = {
+    {16, 32, 48},  {16, 32, 0},                       // (0, 1: k shared by 4 waves, by 2)
+    {64, 32, 60},  {64, 64, 140}, {64, 128, 0},       // (2 - 4)
+    {128, 32, 24}, {128, 64, 56}, {128, 128, 0}};     // (5 - 7)
+constexpr int I8_ODD_COUNT = sizeof(I8_ODD_SHAPES) / sizeof(I8_ODD_SHAPES[0]);
+inline int i8_odd_tile_for(int V, int B, int n_cu) {
+  return i8_shape_for(I8_ODD_SHAPES, I8_ODD_COUNT, B <= 16 ? 16 : B <= 64 ? 64 : 128, V, B, n_cu);
 }

@@ -194,7 +194,7 @@ def test_every_tile(torch_cuda, V):
     g = torch.Generator(device="cuda")
     g.manual_seed(V)
     for B in I8_TILE_BATCHES:
-        for n in (208, 400):
+        for n in (208, 400, 277):  # (277: rows off 16 bytes, shapes of their own)
             w = torch.randint(-128, 128, (V, n), generator=g, device="cuda", dtype=torch.int8)
             xq = torch.randint(-128, 128, (B, n), generator=g, device="cuda", dtype=torch.int8)
             sw = torch.rand(V, generator=g, device="cuda")

@@ -11,11 +11,11 @@ SRC = os.path.join(ROOT, "tests", "native", "i8_tile_check.cpp")
 INC = os.path.join(ROOT, "project-zero_amd", "csrc")
 
 
-def tiles(tmp_path, cases):
+def tiles(tmp_path, cases, *how):
     exe = tmp_path / "i8_tile_check"
     subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-I", INC, SRC, "-o", str(exe)],
                    check=True)
-    out = subprocess.run([str(exe)] + [str(v) for c in cases for v in c], capture_output=True,
+    out = subprocess.run([str(exe), *how] + [str(v) for c in cases for v in c], capture_output=True,
                          text=True, timeout=60, check=True)
     count, *got = [int(v) for v in out.stdout.split()]
     return count, got
@@ -24,6 +24,17 @@ def tiles(tmp_path, cases):
 def test_the_gpu_cases_reach_every_shape(tmp_path):
     count, got = tiles(tmp_path, [(B, V) for B in I8_TILE_BATCHES for V in I8_TILE_VOCABS])
     assert set(got) == set(range(count))
+
+
+def test_the_gpu_cases_reach_every_shape_of_odd_rows(tmp_path):
+    count, got = tiles(tmp_path, [(B, V) for B in I8_TILE_BATCHES for V in I8_TILE_VOCABS], "odd")
+    assert set(got) == set(range(count))
+
+
+def test_the_ends_of_the_rule_of_odd_rows(tmp_path):
+    _, got = tiles(tmp_path, [(1, 1), (16, 2 ** 31 - 1), (17, 1), (64, 2 ** 31 - 1), (65, 1),
+                              (100000, 2 ** 31 - 1)], "odd")
+    assert got == [0, 1, 2, 4, 5, 7]
 
 
 def test_the_ends_of_the_rule(tmp_path):
