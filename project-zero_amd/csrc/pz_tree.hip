@@ -33,7 +33,7 @@
 //
 // k_tree_wide, many rows over many keys: the waves of a workgroup own 16 RT rows each and share
 // the keys, whose tiles come to LDS through a ring of loads.  Bound by issue: 8 x
-// 64 nodes over 32768 positions 343 us (275 GFLOP at 0.80 PFLOP/s, 3.1 TB/s of
+// 64 nodes over 32768 positions 337 us (275 GFLOP at 0.82 PFLOP/s, 3.2 TB/s of
 // keys and values).  Of a tile's 1.3 us a SIMD's two waves take 0.5 for the
 // products, 0.6 for the other vector instructions, and LDS 0.55 for the fragments
 // and the loads; before the fragments were read a phase ahead it was 363 us, 257 of
