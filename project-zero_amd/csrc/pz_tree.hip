@@ -5,8 +5,13 @@
 //   out[r] = sum_p softmax_p(scale q[r] . k[p]) v[p],  r = (node, head of a key
 //   head's group), p over the cached positions and the nodes that r's node sees.
 //
-// One pass over the keys with a running maximum m and sum l per row; the scores'
-// exponentials are taken to base 2 of scale log2(e) s - m.  All rows of a key head
+// One pass over the keys with a running maximum m and sum l per row.  m is a score
+// q . k itself and weights are 2^(c (s - m)), c = scale log2(e).  Where |c m| is at
+// most 2^12 they are taken as fma(s, c, -c m), which half a unit of c m, 2^-12, moves
+// alike for every key.  Farther out that would be a weight of its own (from 2^26 on
+// 2^8 and more), so there s - m comes first: the difference of floats that lie close
+// is exact, and the largest score's weight with it, wherever fp32 holds the scores.
+// (Always so: 8 x 64 nodes over 32768 positions 347 us, 336 so; one fma throughout 333.)  All rows of a key head
 // share its keys, so nodes x group rows meet each tile of 32 keys: 16 of them a
 // column of v_mfma_f32_16x16x32.  Both kernels compute
 //
@@ -68,7 +73,9 @@ constexpr int TR_SHARE = 8;         // tiles that are worth a workgroup
 constexpr int TR_ENTRIES = 2048;    // table entries that the wide kernel keeps in LDS
 constexpr int TR_STAGES = 6;        // tiles of its ring
 constexpr int TR_WIDE = 8;          // its waves
-constexpr float TR_LOW = -3.0e38f;  // m before any score (finite: m - m is 0)
+constexpr float TR_LOW = -3.40282346638528859812e38f;  // m before any score (the least float:
+                                                       // m - m is 0, and no score lies below)
+constexpr float TR_NEAR = 4096.0f;  // largest |c m| whose rounding is none of a weight's business
 constexpr float TR_LOG2E = 1.44269504088896340736f;
 
 template <int TYPE>
@@ -129,7 +136,7 @@ struct TreeArgs {
   long ld_out;
   int S, nblk;  // most splits of a sequence, row blocks of a key head
   int chunk;    // tiles of a split of the longest table
-  float* part;  // [unit][S] results (TR result order), then their m and l
+  float* part;  // [unit][S] results (a lane's order), then their m and l
   float* ml;
 };
 
@@ -172,6 +179,11 @@ __device__ __forceinline__ int tr_chunk(const TreeArgs& A, int b, int lane) {
   return share < TR_SHARE ? TR_SHARE : share;
 }
 
+// What results taken against the maximum m count for against the maximum top.
+__device__ __forceinline__ float tr_lift(float m, float top, float c) {
+  return __builtin_amdgcn_exp2f((m - top) * c);
+}
+
 // A lane's results of one row: d = NT (4 g + i) + 4 f + 0..3 in o (i, f).
 template <int TYPE>
 __device__ __forceinline__ void tr_store4(uint16_t* o, const tr_f32x4 v) {
@@ -188,6 +200,8 @@ struct TrRows {
   static constexpr int KS = D / 32, NT = D / 16, NW = NT / 2;  // k steps, d tiles, words of V
   tr_f32x4 o[RT][NT];
   float mx[RT], l[RT];
+  bool far;      // some row's |c m| is above TR_NEAR: s - m before the fma (wave-uniform)
+  float nb[RT];  // what the fma adds
   tr_f32x4 s[RT][2];  // scores, then weights: keys 16 t + 4 g + i of row m
   int m, g;
   float c;  // scale log2(e)
@@ -196,9 +210,11 @@ struct TrRows {
     m = lane & 15;
     g = lane >> 4;
     c = scale;
+    far = true;
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
       mx[rt] = TR_LOW;
+      nb[rt] = Y::OFF;
       l[rt] = 0.0f;
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) o[rt][nt] = tr_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -252,30 +268,41 @@ struct TrRows {
       tm[rt] = most(most(most(s[rt][0][0], s[rt][0][1]), most(s[rt][0][2], s[rt][0][3])),
                     most(most(s[rt][1][0], s[rt][1][1]), most(s[rt][1][2], s[rt][1][3])));
   }
-  // raises m where a score passes it by far
+  // raises m where a score passes it by 2^TH, and readies the scores for their weights
   __device__ __forceinline__ void raise(const float (&tm)[RT]) {
     bool up = false;
 #pragma unroll
-    for (int rt = 0; rt < RT; rt++) up |= tm[rt] * c > mx[rt] + Y::TH;
+    for (int rt = 0; rt < RT; rt++) up |= (tm[rt] - mx[rt]) * c > Y::TH;
     if (__ballot(up)) {
 #pragma unroll
       for (int rt = 0; rt < RT; rt++) {
-        float t = tm[rt] * c;
+        float t = tm[rt];
         t = fmaxf(t, __shfl_xor(t, 16, 64));
         t = fmaxf(t, __shfl_xor(t, 32, 64));
         const float mn = fmaxf(mx[rt], t);
-        const float al = __builtin_amdgcn_exp2f(mx[rt] - mn);
+        const float al = tr_lift(mx[rt], mn, c);
         mx[rt] = mn;
         l[rt] *= al;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) o[rt][nt] *= al;
       }
+      bool out = false;
+#pragma unroll
+      for (int rt = 0; rt < RT; rt++) out |= !(fabsf(mx[rt] * c) <= TR_NEAR);
+      far = __ballot(out) != 0;
+#pragma unroll
+      for (int rt = 0; rt < RT; rt++) nb[rt] = far ? Y::OFF : Y::OFF - mx[rt] * c;
     }
+    if (far)
+#pragma unroll
+      for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) s[rt][e >> 2][e & 3] -= mx[rt];
   }
-  // weight e of row tile rt from its score
+  // weight e of row tile rt from its score, which raise() has seen
   __device__ __forceinline__ void weigh(int rt, int e) {
-    const float p = __builtin_amdgcn_exp2f(
-        __builtin_fmaf(s[rt][e >> 2][e & 3], c, -(mx[rt] - Y::OFF)));
+    const float p =
+        __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][e >> 2][e & 3], c, nb[rt]));
     s[rt][e >> 2][e & 3] = p;
     l[rt] += p;
   }
@@ -573,8 +600,8 @@ k_tree(const TreeArgs A) {
     lt[rt] = 0.0f;
 #pragma unroll
     for (int i = 0; i < WAVES; i++)
-      lt[rt] += mls[i][rt * 16 + m][1] * __builtin_amdgcn_exp2f(mls[i][rt * 16 + m][0] - mt[rt]);
-    const float al = __builtin_amdgcn_exp2f(R.mx[rt] - mt[rt]);
+      lt[rt] += mls[i][rt * 16 + m][1] * tr_lift(mls[i][rt * 16 + m][0], mt[rt], A.c);
+    const float al = tr_lift(R.mx[rt], mt[rt], A.c);
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) R.o[rt][nt] *= al;
   }
@@ -1007,13 +1034,13 @@ __global__ __launch_bounds__(64 * TR_JOIN) void k_tree_join(const TreeArgs A) {
     float mn = mt;
 #pragma unroll
     for (int u = 0; u < U; u++) mn = fmaxf(mn, ms[u]);
-    const float al = __builtin_amdgcn_exp2f(mt - mn);
+    const float al = tr_lift(mt, mn, A.c);
     mt = mn;
     lt *= al;
     o *= al;
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const float e = __builtin_amdgcn_exp2f(ms[u] - mt);
+      const float e = tr_lift(ms[u], mt, A.c);
       lt += ls[u] * e;
       if (s0 + u * WAVES < ns) o += v[u] * e;
     }
@@ -1030,12 +1057,12 @@ __global__ __launch_bounds__(64 * TR_JOIN) void k_tree_join(const TreeArgs A) {
     float mx = mt;
 #pragma unroll
     for (int k = 1; k < WAVES; k++) mx = fmaxf(mx, mls[k][m][0]);
-    const float a0 = __builtin_amdgcn_exp2f(mt - mx);
+    const float a0 = tr_lift(mt, mx, A.c);
     lt *= a0;
     o *= a0;
 #pragma unroll
     for (int k = 1; k < WAVES; k++) {
-      const float e = __builtin_amdgcn_exp2f(mls[k][m][0] - mx);
+      const float e = tr_lift(mls[k][m][0], mx, A.c);
       lt += mls[k][m][1] * e;
       o += sum[k][lane] * e;
     }
