@@ -179,6 +179,19 @@ __device__ __forceinline__ int tr_chunk(const TreeArgs& A, int b, int lane) {
   return share < TR_SHARE ? TR_SHARE : share;
 }
 
+// One over the sum l of the weights of node t's row.  A sum of 0 is a row that attends
+// nothing, whose result is zeros, or one whose every score is -infinity, which is NaN.
+__device__ __forceinline__ float tr_inverse(const TreeArgs& A, int b, int t, float l) {
+  if (l != 0.0f) return 1.0f / l;
+  const uint64_t sees = A.tree ? A.tree[(size_t)b * A.T + t] : ~0ull;
+  if (sees << (64 - tr_nodes(A, b))) return __builtin_nanf("");
+  const int ctx = pz_pages_len(A.pages, A.len[b]);
+  for (int e = 0; (int64_t)e << A.pages.shift < ctx; e++)
+    if ((uint32_t)A.blocks[(size_t)b * A.pages.max_blocks + e] < (uint32_t)A.pages.n_blocks)
+      return __builtin_nanf("");
+  return 0.0f;
+}
+
 // What results taken against the maximum m count for against the maximum top.
 __device__ __forceinline__ float tr_lift(float m, float top, float c) {
   return __builtin_amdgcn_exp2f((m - top) * c);
@@ -648,9 +661,8 @@ k_tree(const TreeArgs A) {
       float lr = lt[0];
 #pragma unroll
       for (int k = 1; k < RT; k++) lr = rt == k ? lt[k] : lr;
-      // nothing seen: l is 0 and so is the result
-      const float inv = lr == 0.0f ? 0.0f : 1.0f / lr;
       const int t = r / A.group, hq = h * A.group + (r - t * A.group);
+      const float inv = tr_inverse(A, b, t, lr);
       tr_store4<TYPE>(A.out + ((size_t)b * A.T + t) * A.ld_out + (size_t)hq * D + 4 * NT * g +
                           NT * i + 4 * f,
                       v * inv);
@@ -976,9 +988,8 @@ k_tree_wide(const TreeArgs A) {
     } else if (r >= rows) {
       continue;
     }
-    // nothing seen: l is 0 and so is the result
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const int t = r / A.group, hq = h * A.group + (r - t * A.group);
+    const float inv = ns > 1 ? 0.0f : tr_inverse(A, b, t, l);
     uint16_t* out = A.out + ((size_t)b * A.T + t) * A.ld_out + (size_t)hq * D + 4 * NT * g;
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -1068,8 +1079,8 @@ __global__ __launch_bounds__(64 * TR_JOIN) void k_tree_join(const TreeArgs A) {
     }
   }
   if (r >= rows) return;
-  const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
   const int t = r / A.group, hq = h * A.group + (r - t * A.group);
+  const float inv = tr_inverse(A, b, t, lt);
   tr_store4<TYPE>(A.out + ((size_t)b * A.T + t) * A.ld_out + (size_t)hq * D + 4 * NT * g + NT * i +
                       4 * f,
                   o * inv);

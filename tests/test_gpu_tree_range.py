@@ -132,3 +132,38 @@ def test_scores_around_the_choice(torch_cuda, sampler, kind, form):
     at = c.slots(0, torch_cuda.arange(int(c.lens[0])))
     k[at] = (torch_cuda.arange(len(at)) * 200 // len(at) - 100).to(c.dt)[:, None]
     c.check(call(sampler, c, 1.0))
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("pages", ["all", "none", "last"])
+def test_scores_of_minus_infinity(torch_cuda, sampler, kind, form, pages):
+    """What a row attends with a score of -infinity takes no weight beside a
+    finite score; a row that attends nothing else is NaN (the quotient of zeros
+    that the formula gives), one that attends nothing is zeros."""
+    torch = torch_cuda
+    c = case(torch, kind, form, 64, 8)
+    if c.B > 1:
+        c.lens[1] = 0
+    q, kn, k = only_first(c)
+    q[:] = 1.0
+    k[:] = -float("inf")
+    kn[:] = 0.0
+    kn[:, ::3] = -float("inf")
+    c.tree[:, 2::3] = 0  # (these see the cache alone)
+    if pages != "all":
+        keep = c.table.clone()
+        c.table[:] = -1
+        if pages == "last":
+            for b in range(c.B):
+                last = max(int(c.lens[b]) - 1, 0) // 16
+                c.table[b, last] = keep[b, last]
+    got = call(sampler, c).reshape(c.B, c.T, c.kv, -1, 64).cpu()
+    for b in range(c.B):
+        assert torch.isnan(got[b, ::3]).all(), b
+        value = c.vn[b].reshape(c.T, c.kv, 1, 64)[1::3]
+        assert torch.equal(got[b, 1::3], value.expand_as(got[b, 1::3])), b
+        if c.lens[b] > 0 and pages != "none":
+            assert torch.isnan(got[b, 2::3]).all(), b
+        else:
+            assert (got[b, 2::3] == 0).all(), b
