@@ -84,6 +84,7 @@ template <>
 struct TrType<PZ_BF16> {
   static constexpr float OFF = 0.0f, TH = 8.0f;
   static constexpr uint32_t EXP = 0x7f80u;  // exponent bits of one element
+  static constexpr float MOST = 3.38953138925153547590e38f;  // its largest
   __device__ __forceinline__ static tr_f32x4 mfma(tr_u32x4 a, tr_u32x4 b, tr_f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(tr_bf16x8, a),
                                                    __builtin_bit_cast(tr_bf16x8, b), c, 0, 0, 0);
@@ -102,6 +103,7 @@ struct TrType<PZ_F16> {
   // their bits (fp16 has normal numbers down to 2^-14)
   static constexpr float OFF = 8.0f, TH = 6.0f;
   static constexpr uint32_t EXP = 0x7c00u;
+  static constexpr float MOST = 65504.0f;
   __device__ __forceinline__ static tr_f32x4 mfma(tr_u32x4 a, tr_u32x4 b, tr_f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(tr_f16x8, a),
                                                   __builtin_bit_cast(tr_f16x8, b), c, 0, 0, 0);
@@ -197,9 +199,16 @@ __device__ __forceinline__ float tr_lift(float m, float top, float c) {
   return __builtin_amdgcn_exp2f((m - top) * c);
 }
 
-// A lane's results of one row: d = NT (4 g + i) + 4 f + 0..3 in o (i, f).
+// A lane's results of one row: d = NT (4 g + i) + 4 f + 0..3 in o (i, f).  A mean of
+// finite values does not pass the type's largest; the rounded weights, whose sum is
+// taken before, can make it do so by 2^-11 (fp16) or 2^-8, which would be an infinity.
 template <int TYPE>
-__device__ __forceinline__ void tr_store4(uint16_t* o, const tr_f32x4 v) {
+__device__ __forceinline__ void tr_store4(uint16_t* o, tr_f32x4 v) {
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    v[i] = fabsf(v[i]) > TrType<TYPE>::MOST && fabsf(v[i]) < __builtin_inff()
+               ? __builtin_copysignf(TrType<TYPE>::MOST, v[i])
+               : v[i];
   tr_u32x2 w;
   w[0] = TrType<TYPE>::pack(v[0], v[1]);
   w[1] = TrType<TYPE>::pack(v[2], v[3]);

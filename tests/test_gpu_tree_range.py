@@ -167,3 +167,30 @@ def test_scores_of_minus_infinity(torch_cuda, sampler, kind, form, pages):
             assert torch.isnan(got[b, 2::3]).all(), b
         else:
             assert (got[b, 2::3] == 0).all(), b
+
+
+def most_of(torch, c):
+    return torch.finfo(c.dt).max
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+def test_saturated_values(torch_cuda, sampler, form):
+    """fp16 values of +-65504 throughout, one key with most of the weight, whose
+    rounding differs from row to row: a mean of such values is one of them, and
+    must not become infinite by the weights' rounding."""
+    torch = torch_cuda
+    c = case(torch, "fp16", form, 64, 9)
+    q, kn, k = only_first(c)
+    q[:] = 1.0 + (torch.arange(q.numel()) % 80 / 1024.0).reshape(q.shape).to(c.dt)
+    kn[:] = -1000.0
+    k[:] = -1000.0
+    for b in range(c.B):
+        at = torch.arange(int(c.lens[b]))
+        k[c.slots(b, at[::32])] = 0.0
+        if len(at):
+            k[c.slots(b, at[len(at) - 1 - len(at) // 5:][:1])] = 5.5
+    sign = torch.randint(0, 2, (64,), generator=torch.Generator().manual_seed(9)) * 2 - 1
+    top = sign.to(c.dt) * most_of(torch, c)
+    for v in (c.v, c.vn):
+        v[:] = top.repeat(c.kv)
+    c.check(call(sampler, c, float(np.log(2.0))))
