@@ -471,11 +471,12 @@ typedef struct {
  * with 0 < scale <= 2e38.
  * q row (b, t) at d_q + (b * T + t) * ld_q, n_heads x head_dim elements; out
  * alike with ld_out.  Sums and softmax in fp32; softmax weights are rounded
- * to the type before they meet the values, the result once more.  A node that
- * attends nothing gets zeros, one whose every score is -infinity NaN; what a
- * node does not attend has no influence, NaN included; rows of nodes from n_b on are left as they are.  ld_q, ld_n
- * and ld_out multiples of 8, pointers 16-byte aligned.  The host sees the
- * tables' length (max_blocks * block_size) and chooses a kernel by it; the
+ * to the type before they meet the values, the result once more, to a finite
+ * value where all values are finite.  A node that attends nothing gets zeros,
+ * one whose every score is -infinity NaN; what a node does not attend has no
+ * influence, NaN included; rows of nodes from n_b on are left as they are.
+ * ld_q, ld_n and ld_out multiples of 8, pointers 16-byte aligned.  The host sees
+ * the tables' length (max_blocks * block_size) and chooses a kernel by it; the
  * kernel shares the work out by the longest sequence's, so tables may be kept
  * larger than needed.  Long sequences are split over workgroups, in a
  * workspace that the first call allocates (64 MiB, kept until the sampler is

@@ -82,7 +82,10 @@ template <int TYPE>
 struct TrType;
 template <>
 struct TrType<PZ_BF16> {
-  static constexpr float OFF = 0.0f, TH = 8.0f;
+  // the weights lie around 2^-40, so that the sums of any 2^31 of them times bf16's
+  // largest values stay in fp32 (which has as many exponents: down there the small
+  // ones keep their bits to 2^-86 of the largest)
+  static constexpr float OFF = -40.0f, TH = 8.0f;
   static constexpr uint32_t EXP = 0x7f80u;  // exponent bits of one element
   static constexpr float MOST = 3.38953138925153547590e38f;  // its largest
   __device__ __forceinline__ static tr_f32x4 mfma(tr_u32x4 a, tr_u32x4 b, tr_f32x4 c) {

@@ -194,3 +194,31 @@ def test_saturated_values(torch_cuda, sampler, form):
     for v in (c.v, c.vn):
         v[:] = top.repeat(c.kv)
     c.check(call(sampler, c, float(np.log(2.0))))
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+def test_the_largest_bf16_values(torch_cuda, sampler, form):
+    """bf16 values of +-3.39e38 throughout: sums of weighted values stay in
+    fp32, and the mean is finite."""
+    torch = torch_cuda
+    c = case(torch, "bf16", form, 64, 10)
+    sign = torch.randint(0, 2, (64,), generator=torch.Generator().manual_seed(10)) * 2 - 1
+    top = sign.to(c.dt) * most_of(torch, c)
+    for v in (c.v, c.vn):
+        v[:] = top.repeat(c.kv)
+    c.check(call(sampler, c))
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+def test_small_bf16_values(torch_cuda, sampler, form):
+    """Values around 2^-90, whose weighted sums are small: the bound of ordinary
+    values, scaled, and half of fp32's least step (2^-150) for each product and
+    partial sum, over a normaliser of at least 2^-40."""
+    torch = torch_cuda
+    c = case(torch, "bf16", form, 64, 11)
+    small = 2.0 ** -90
+    c.v, c.vn = (v * small for v in (c.v, c.vn))  # (a power of two: exact)
+    got = call(sampler, c).reshape(c.B, c.T, c.heads, 64).double().cpu().numpy()
+    exp, tol = c.want()
+    tol = tol + 2 * (int(c.lens.max()) + c.T) * 2.0 ** -110
+    assert (np.abs(got - exp) <= tol).all(), (np.abs(got - exp) / tol).max()
