@@ -418,7 +418,8 @@ PZ_API int pz_quant_rows_i8(pz_sampler *s, const void *d_x, int x_type, long ldx
  * device [B, ldx] int8 with a scale per row (token) in d_sx [B].  The sum is
  * exact (int32; n <= PZ_I8_MAX_N, PZ_ERANGE beyond), so every logit is the
  * formula's to the bit, in any batch.  Half the bytes of pz_lm_head_bf16's
- * weights.  B <= max_batch.  Rows of d_w and d_x that start 16-byte aligned
+ * weights.  B <= max_batch, V <= 2^30 and no more tiles than a launch takes
+ * (PZ_ERANGE beyond).  Rows of d_w and d_x that start 16-byte aligned
  * (n and ldx multiples of 16) are the quick case.  Asynchronous on the
  * sampler's stream. */
 #define PZ_I8_MAX_N 131071

@@ -570,12 +570,14 @@ template <int WR, int WC, int WK, int TR, int TC, int NS, int NX, int MODE, bool
 int launch(pz_sampler* s, const I8Call& c) {
   constexpr int rows = WR * TR * 16, cols = WC * TC * 16;
   const int ncb = (c.B + cols - 1) / cols, nrt = (c.V + rows - 1) / rows;
-  const unsigned grid = (unsigned)((nrt + 7) / 8 * 8) * ncb;
+  const int64_t grid = i8_workgroups(c.V, c.B, rows, cols);
+  if (!pz_launch_fits(grid, 64 * WR * WC * WK))
+    return fail(s, PZ_ERANGE, "V=%d x B=%d are more tiles than a launch takes", c.V, c.B);
   // weights past the Infinity Cache are not kept (lm_once counts bf16 weights)
   auto k = FAST && lm_once(c.V, (c.n + 1) / 2)
                ? k_lmhead_i8<WR, WC, WK, TR, TC, NS, NX, MODE, FAST, FAST>
                : k_lmhead_i8<WR, WC, WK, TR, TC, NS, NX, MODE, FAST, false>;
-  hipLaunchKernelGGL(k, dim3(grid), dim3(64 * WR * WC * WK), 0, s->stream, c.w, c.sw, c.V, c.n, c.x,
+  hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(64 * WR * WC * WK), 0, s->stream, c.w, c.sw, c.V, c.n, c.x,
                      c.sx, c.ldx, c.B, ncb, nrt, c.out, c.ld, s->d_lmh_keys, s->max_batch,
                      s->d_lmh_nan);
   PZ_HIP(s, hipGetLastError());

@@ -1,6 +1,7 @@
 // pz_lmtile.h -- which LM-head path and tile shape a call takes (host only).
 #pragma once
 #include <stddef.h>
+#include <stdint.h>
 
 // Weights the Infinity Cache (256 MB) cannot hold from one call to the next
 // are loaded non-temporally: 128256 x 2560 at batch 1 114 -> 98 us, at 8
@@ -83,6 +84,12 @@ inline int i8_shape_for(const I8Tile* shapes, int count, int cols, int V, int B,
   for (int i = 0; i < count; i++)
     if (shapes[i].cols == cols && (shapes[i].most == 0 || rows <= shapes[i].most)) return i;
   return count - 1;
+}
+// Workgroups of a launch of tiles of `rows` x `cols`: the row tiles in eights, one
+// for each XCD.
+inline int64_t i8_workgroups(int V, int B, int rows, int cols) {
+  const int64_t nrt = ((int64_t)V + rows - 1) / rows, ncb = ((int64_t)B + cols - 1) / cols;
+  return (nrt + 7) / 8 * 8 * ncb;
 }
 inline int i8_tile_for(int V, int B, int n_cu) {
   const int cols = B <= 16 ? 16 : B <= 32 ? 32 : B <= 64 ? 64 : B <= 128 ? 128 : 256;

@@ -57,6 +57,7 @@ inline PzRefusal pz_refuse_i8(const int8_t* d_w, const float* d_sw, int V, int n
   if (!d_w || !d_sw || !d_x || !d_sx || V <= 0 || n <= 0 || B < 0 || ldx < n)
     return {PZ_EINVAL, "bad LM head shape"};
   if (n > PZ_I8_MAX_N) return {PZ_ERANGE, "n > PZ_I8_MAX_N: the sum does not fit 32 bits"};
+  if (V > PZ_MOST) return {PZ_ERANGE, "V above 2^30"};
   if (B > max_batch) return {PZ_ERANGE, "B > max_batch"};
   return PZ_TAKEN;
 }
