@@ -56,6 +56,7 @@
 #include "pz_pages.h"
 #include "pz_refuse.h"
 #include "pz_sampler_impl.h"
+#include "pz_treeplan.h"
 
 namespace {
 
@@ -1173,31 +1174,14 @@ int run_rows(pz_sampler* s, TreeArgs& A) {
     const int64_t want = (s->n_cu + wgs - 1) / wgs, most = tiles / TR_SHARE;
     return want < most ? want : most;
   };
-  if (rows <= 16) {
-    // Few short sequences: eight waves and no launch to join.  (One token over 500
-    // positions 11.5 us, 12.0 in splits of four waves, 16 sequences 12.7 / 15.1; but
-    // over 1000 15.1 / 11.8, and 512 key heads 34.0 / 29.9.)  Heads of 256 spill
-    // there: 500 positions 20.2 us, in splits 16.1.
-    if constexpr (D < 256)
-      if (tiles <= 24 && heads <= s->n_cu) return narrow<TYPE, D, 1, 8>(s, A, tiles, 1);
-    return narrow<TYPE, D, 1, 4>(s, A, tiles, splits(heads));
-  }
-  // The wide kernel (us, narrow / wide of 16 rows a wave / of 32):
-  //   32 ragged sequences of up to 4096 positions x 8 key heads: 20 rows 73 / 74; 32
-  //   74 / 76; 48 97 / 78 / 90; 64 - / 78 / 90; 96 - / 95 / 90; 128 - / 105 / 91; 256 -
-  //   / 181 / 142: from 33 rows on, and 16 a wave while each has a SIMD.
-  //   256 rows, 8 sequences x 8 key heads, by positions: 500 22 / - / 38; 1000 31 / -
-  //   / 40; 2000 51 / - / 50; 4000 96 / - / 73; one sequence 2000 18 / - / 25, 8000 33
-  //   / - / 34, 16000 49 / - / 41; 48 rows 8000 16 / 17, 32768 41 / 36: from 16
-  //   tiles a CU on, below which k_tree's row blocks fill more CUs; but with a
-  //   workgroup for each CU at once (32 x 8) 100 47 / - / 35, 48 rows 250 17 / 15.
+  const TrKernel kernel = tr_kernel_for(rows, heads, tiles, s->n_cu, D, A.ld, A.ld_n);
   if constexpr (D < 256) {
-    // (its offsets within a load's rows are 32 bits)
-    if (rows > 32 && (heads >= s->n_cu || heads * tiles >= 16 * s->n_cu) && A.ld < (1 << 26) &&
-        A.ld_n < (1 << 24))
-      return rows <= 64 ? wide<TYPE, D, 1>(s, A, tiles, splits(heads))
-                        : wide<TYPE, D, 2>(s, A, tiles, splits(heads * ((rows + 255) / 256)));
+    if (kernel == TR_FEW_SHORT) return narrow<TYPE, D, 1, 8>(s, A, tiles, 1);
+    if (kernel == TR_WIDE16) return wide<TYPE, D, 1>(s, A, tiles, splits(heads));
+    if (kernel == TR_WIDE32)
+      return wide<TYPE, D, 2>(s, A, tiles, splits(heads * ((rows + 255) / 256)));
   }
+  if (kernel == TR_FEW) return narrow<TYPE, D, 1, 4>(s, A, tiles, splits(heads));
   return narrow<TYPE, D, 2, 4>(s, A, tiles, splits(heads * ((rows + 31) / 32)));
 }
 
