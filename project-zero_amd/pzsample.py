@@ -234,7 +234,10 @@ def _params_array(params, B):
 
 
 class Sampler:
-    """One pz_sampler (stream + scratch + staging) on one device."""
+    """One pz_sampler (stream + scratch + staging) on one device.
+
+    The asynchronous calls work on their device buffers until sync(): the caller
+    keeps them, and writes none that a call reads, till then."""
 
     def __init__(self, max_batch, max_vocab, max_hist=0, device=0,
                  temp_mode=PZ_TEMP_MUL_RECIP):
