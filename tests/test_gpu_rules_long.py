@@ -5,7 +5,7 @@ import pytest
 
 import pzsample as pz
 from conftest import to_dev
-from test_gpu_rules import F, PENS, logits, run, same
+from test_gpu_rules import F, PENS, logits, pack, run, same, want
 
 pytestmark = pytest.mark.gpu
 
@@ -67,3 +67,40 @@ def test_long_lists_of_repeated_ids_with_every_rule(torch_cuda):
     for mask in (None, on):
         for inplace in (True, False):
             run(torch_cuda, x, V, PENS[3], None, hist, None, bid, bias, mask, None, inplace)
+
+
+@pytest.mark.parametrize("H", [70, 1 << 30])
+@pytest.mark.parametrize("inplace", [True, False])
+def test_rows_past_32_bits(torch_cuda, H, inplace):
+    """Three rows 2^30 elements apart, of logits, masks and (the longer ones)
+    histories: the last lie past 2^31 elements."""
+    torch = torch_cuda
+    V, far = 4100, 1 << 30
+    rng = np.random.default_rng(9)
+    x = logits(3, V, 9)
+    hist = rng.integers(-1, V, (3, 70), dtype=np.int32)
+    lens = np.array([70, 40, 69], np.int32)
+    bid = rng.integers(-1, V, (3, 9), dtype=np.int32)
+    bias = logits(3, 9, 10)
+    on = rng.random((3, V)) < 0.7
+
+    def spread(a, ld):
+        pool = torch.empty(2 * ld + a.shape[1], dtype=torch.from_numpy(a).dtype, device="cuda")
+        pool.as_strided(a.shape, (ld, 1)).copy_(torch.from_numpy(a))
+        return pool
+
+    words = pack(on).view(np.int32)
+    d_x, d_mask = spread(x, far), spread(words, far)
+    d_hist = spread(hist, H) if H > 70 else to_dev(torch, hist)
+    d_out = d_x if inplace else spread(np.zeros_like(x), far + 3)
+    d_allowed = torch.empty(3, dtype=torch.int32, device="cuda")
+    rules = pz.logit_rules(*PENS[3], d_hist=d_hist, H=H, d_hist_len=to_dev(torch, lens),
+                           d_bias_ids=to_dev(torch, bid), d_bias=to_dev(torch, bias), n_bias=9,
+                           d_mask=d_mask, ld_mask=far, n_masks=3, d_allowed=d_allowed)
+    ld_out = far if inplace else far + 3
+    with pz.Sampler(1, 16) as s:
+        s.rules(d_x, d_out, 3, V, far, ld_out, rules)
+        s.sync()
+    exp, allowed = want(x, V, [PENS[3]] * 3, hist, lens, bid, bias, on)
+    same(d_out.as_strided((3, V), (ld_out, 1)).cpu().numpy(), exp, (H, inplace))
+    assert (d_allowed.cpu().numpy() == allowed).all()
