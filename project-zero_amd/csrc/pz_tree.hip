@@ -6,12 +6,14 @@
 //   head's group), p over the cached positions and the nodes that r's node sees.
 //
 // One pass over the keys with a running maximum m and sum l per row.  m is a score
-// q . k itself and weights are 2^(c (s - m)), c = scale log2(e).  Where |c m| is at
-// most 2^12 they are taken as fma(s, c, -c m), which half a unit of c m, 2^-12, moves
-// alike for every key.  Farther out that would be a weight of its own (from 2^26 on
-// 2^8 and more), so there s - m comes first: the difference of floats that lie close
-// is exact, and the largest score's weight with it, wherever fp32 holds the scores.
-// (Always so: 8 x 64 nodes over 32768 positions 347 us, 336 so; one fma throughout 333.)  All rows of a key head
+// q . k itself and weights are 2^(c (s - m)), c = scale log2(e): the difference of
+// floats that lie close is exact, and the largest score's weight with it, wherever
+// fp32 holds the scores.  (One fma(s, c, -c m) moves the weights by half a unit of
+// c m, alike for every key of a tile, but from 2^26 on that is 2^8 and more.)  k_tree,
+// which memory bounds, always subtracts; k_tree_wide takes the fma where |c m| is at
+// most 2^12, half a unit 2^-12 (8 x 64 nodes over 32768 positions: 333 us with the fma
+// alone, 336 so, 347 with the difference alone; in k_tree the choice costs heads of
+// 256 registers that they lack, 32 ragged x 5 nodes 148 us for 125).  All rows of a key head
 // share its keys, so nodes x group rows meet each tile of 32 keys: 16 of them a
 // column of v_mfma_f32_16x16x32.  Both kernels compute
 //
@@ -220,14 +222,15 @@ __device__ __forceinline__ void tr_store4(uint16_t* o, tr_f32x4 v) {
 }
 
 // The running state of 16 RT rows in one wave, and the steps of one tile of keys.
-template <int TYPE, int D, int RT>
+// CHOOSE: weights by one fma where every |c m| is small, else always from s - m.
+template <int TYPE, int D, int RT, bool CHOOSE>
 struct TrRows {
   typedef TrType<TYPE> Y;
   static constexpr int KS = D / 32, NT = D / 16, NW = NT / 2;  // k steps, d tiles, words of V
   tr_f32x4 o[RT][NT];
   float mx[RT], l[RT];
-  bool far;      // some row's |c m| is above TR_NEAR: s - m before the fma (wave-uniform)
-  float nb[RT];  // what the fma adds
+  bool far;      // (CHOOSE) some row's |c m| is above TR_NEAR: s - m first (wave-uniform)
+  float nb[RT];  // (CHOOSE) what the fma adds
   tr_f32x4 s[RT][2];  // scores, then weights: keys 16 t + 4 g + i of row m
   int m, g;
   float c;  // scale log2(e)
@@ -312,14 +315,16 @@ struct TrRows {
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) o[rt][nt] *= al;
       }
-      bool out = false;
+      if (CHOOSE) {
+        bool out = false;
 #pragma unroll
-      for (int rt = 0; rt < RT; rt++) out |= !(fabsf(mx[rt] * c) <= TR_NEAR);
-      far = __ballot(out) != 0;
+        for (int rt = 0; rt < RT; rt++) out |= !(fabsf(mx[rt] * c) <= TR_NEAR);
+        far = __ballot(out) != 0;
 #pragma unroll
-      for (int rt = 0; rt < RT; rt++) nb[rt] = far ? Y::OFF : Y::OFF - mx[rt] * c;
+        for (int rt = 0; rt < RT; rt++) nb[rt] = far ? Y::OFF : Y::OFF - mx[rt] * c;
+      }
     }
-    if (far)
+    if (CHOOSE && far)
 #pragma unroll
       for (int rt = 0; rt < RT; rt++)
 #pragma unroll
@@ -327,8 +332,8 @@ struct TrRows {
   }
   // weight e of row tile rt from its score, which raise() has seen
   __device__ __forceinline__ void weigh(int rt, int e) {
-    const float p =
-        __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][e >> 2][e & 3], c, nb[rt]));
+    const float d = CHOOSE ? s[rt][e >> 2][e & 3] : s[rt][e >> 2][e & 3] - mx[rt];
+    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(d, c, CHOOSE ? nb[rt] : Y::OFF));
     s[rt][e >> 2][e & 3] = p;
     l[rt] += p;
   }
@@ -552,7 +557,7 @@ k_tree(const TreeArgs A) {
   }
   __syncthreads();
 
-  TrRows<TYPE, D, RT> R;
+  TrRows<TYPE, D, RT, false> R;
   R.clear(lane, A.c);
   auto scores = [&]() {
     R.scores([&](int t, int ks) { return kf[t][ks]; },
@@ -695,7 +700,7 @@ template <int TYPE, int D, int RT>
 __global__ __launch_bounds__(64 * TR_WIDE) __attribute__((amdgpu_waves_per_eu(TR_WIDE / 4, 8))) void
 k_tree_wide(const TreeArgs A) {
   constexpr int WAVES = TR_WIDE, NS = TR_STAGES;
-  typedef TrRows<TYPE, D, RT> Rows;
+  typedef TrRows<TYPE, D, RT, true> Rows;
   constexpr int KS = D / 32, NT = D / 16, NW = NT / 2, ROWS = 16 * RT, CH = RT * NT;
   constexpr int TILE = TR_KEYS * D * 2;            // bytes of a tile's keys, or of its values
   constexpr int LN = TILE / 1024, PER = 2 * LN / WAVES;  // 1 KiB loads: of a tile's keys, of a wave
