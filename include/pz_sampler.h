@@ -476,12 +476,14 @@ typedef struct {
  * value where all values are finite.  A node that attends nothing gets zeros,
  * one whose every score is -infinity NaN; what a node does not attend has no
  * influence, NaN included; rows of nodes from n_b on are left as they are.
- * ld_q, ld_n and ld_out multiples of 8, pointers 16-byte aligned.  The host sees
- * the tables' length (max_blocks * block_size) and chooses a kernel by it; the
- * kernel shares the work out by the longest sequence's, so tables may be kept
- * larger than needed.  Long sequences are split over workgroups, in a
- * workspace that the first call allocates (64 MiB, kept until the sampler is
- * destroyed).
+ * (An infinite value whose weight rounds to 0 gives NaN.)  ld_q, ld_n and ld_out
+ * multiples of 8, pointers 16-byte aligned.  The host sees the tables' length
+ * (max_blocks * block_size), not the sequences', and chooses a kernel by it.
+ * Where sequences times key heads (and blocks of rows) do not fill the compute
+ * units, long sequences are split over workgroups, each a share of the longest
+ * one there is, in a workspace that the first call allocates (64 MiB, kept
+ * until the sampler is destroyed); where they do, nothing is split, and the
+ * call takes as long as its longest sequence.
  * Asynchronous on the sampler's stream; after that first call it can be
  * captured into a HIP graph.  Calls of one sampler, replays included, must be
  * ordered (on one stream or by events): they share the workspace. */
