@@ -430,7 +430,8 @@ PZ_API int pz_lm_head_i8(pz_sampler *s, const int8_t *d_w, const float *d_sw, in
 /* The same product with greedy sampling fused into its epilogue, as
  * pz_lm_head_argmax_bf16: d_ids[b] is the argmax of exactly the logits
  * pz_lm_head_i8 writes (the first maximum; a NaN logit 0 gives 0).
- * Asynchronous on the sampler's stream. */
+ * Asynchronous on the sampler's stream.  Fused calls of one sampler, replays
+ * included, must be ordered: they share the keys of their maxima. */
 PZ_API int pz_lm_head_argmax_i8(pz_sampler *s, const int8_t *d_w, const float *d_sw, int V, int n,
                                 const int8_t *d_x, const float *d_sx, int B, long ldx,
                                 int32_t *d_ids);
