@@ -504,6 +504,141 @@ PZ_API int pz_cache_append(pz_sampler *s, const pz_kv_cache *cache, const void *
                            const void *d_vn, long ld_n, int B, int T, const int32_t *d_take,
                            const int32_t *d_count);
 
+/* Keys that several sequences share: a prompt and its beams, a system prompt and
+ * the batch under it.  Prefix i holds d_len[i] positions (clamped to [0, max_blocks *
+ * block_size]) in the pages d_blocks[i, ...] of the cache that it is used with
+ * ([n_prefixes, max_blocks] page numbers, as that cache's own tables).  Sequences
+ * d_first[i] .. d_first[i + 1] - 1 have prefix i (d_first: device [n_prefixes + 1],
+ * ascending, values outside [0, B] clamped; a sequence outside every range has none;
+ * where ranges overlap, the results of their sequences are unspecified); NULL: B /
+ * n_prefixes each, in order (n_prefixes must then divide B). */
+typedef struct {
+  const int32_t *d_blocks;
+  int max_blocks;
+  const int32_t *d_len;
+  int n_prefixes;
+  const int32_t *d_first;
+} pz_kv_prefix;
+
+/* pz_tree_attention with a prefix before each sequence's own cache, read once for
+ * the sequences that share it: node t of sequence b attends the positions of b's
+ * prefix, then the d_len[b] positions of its own pages and the nodes that it sees, as
+ * one softmax.  Arguments, results, rounding and refusals as pz_tree_attention (a
+ * softmax weight is rounded against the largest score of the keys that its workgroup
+ * reads); also, T * n_heads is at most 32768.  All sequences' rows of a key head meet
+ * the prefix's keys together, so that its bytes do not grow with the sequences.
+ * Asynchronous on the sampler's stream, in pz_tree_attention's workspace, which the
+ * first call of either allocates; after that call it can be captured into a HIP
+ * graph.  Calls of both on one sampler, replays included, must be ordered. */
+PZ_API int pz_prefix_attention(pz_sampler *s, const pz_kv_cache *cache,
+                               const pz_kv_prefix *prefix, const void *d_kn, const void *d_vn,
+                               long ld_n, int B, int T, const int32_t *d_n_nodes,
+                               const uint64_t *d_tree, int n_heads, float scale, const void *d_q,
+                               long ld_q, void *d_out, long ld_out);
+
+/* What pz_qk_norm_rope does to a head of head_dim elements (at most 1024):
+ *   norm: y = x * w / sqrt(mean(x^2) + eps), w = d_q_norm or d_k_norm (device
+ *     [head_dim]; NULL: y = x, for queries and keys on their own);
+ *   rotation of y's first rot_dim elements (even, 0 .. head_dim; the others are
+ *     left), pair i by the angle pos * d_freq[i] (device [rot_dim / 2], radians a
+ *     position: whatever scaling of long contexts the model has is in these):
+ *       (a, b) -> (a cos - b sin, b cos + a sin) * amplitude
+ *     where pair i is elements i and i + rot_dim / 2 (PZ_ROPE_HALVES) or 2 i and
+ *     2 i + 1 (PZ_ROPE_PAIRS). */
+#define PZ_ROPE_HALVES 0
+#define PZ_ROPE_PAIRS  1
+typedef struct {
+  int type; /* of the rows in and out: PZ_F32, PZ_BF16, PZ_F16 */
+  int n_heads;
+  int n_kv_heads;
+  int head_dim;
+  const float *d_q_norm;
+  const float *d_k_norm;
+  float eps;
+  int rot_dim;
+  int layout;
+  const float *d_freq;
+  float amplitude; /* 1: a rotation */
+} pz_qk_rope;
+
+/* Norms of the queries' and keys' heads and their rotation to the tokens'
+ * positions, in one pass between the projection and pz_tree_attention,
+ * pz_prefix_attention and pz_cache_append: token r's n_heads queries at d_q + r *
+ * ld_q and n_kv_heads keys at d_k + r * ld_k go to d_q_out + r * ld_q_out and
+ * d_k_out + r * ld_k_out (strides in elements).  d_pos: device [n] positions.  In
+ * fp32, the angles in 64 bits, one rounding to the type at the end.  The rows of q
+ * and k may be parts of one row (of a fused projection).  d_q_out == d_q with equal
+ * strides works in place, and d_k_out == d_k alike; outputs must not overlap the
+ * inputs otherwise.  Without queries (n_heads = 0, d_q and d_q_out NULL) or without
+ * keys alike.  Pointers and strides that are multiples of 16 bytes, and rot_dim / 2
+ * (PZ_ROPE_HALVES) and head_dim likewise, are the quick case.  Asynchronous on the
+ * sampler's stream; uses no workspace and can be captured into a HIP graph. */
+PZ_API int pz_qk_norm_rope(pz_sampler *s, const pz_qk_rope *rope, const void *d_q, long ld_q,
+                           const void *d_k, long ld_k, void *d_q_out, long ld_q_out,
+                           void *d_k_out, long ld_k_out, int n, const int32_t *d_pos);
+
+/* One selection of a beam search.  Group g has W beams (at most PZ_BEAM_MAX_WIDTH),
+ * rows g * W .. g * W + W - 1 of d_logits [n_groups * W, ld], whose hypotheses have
+ * the scores d_scores [n_groups * W] (sums of log probabilities) so far.  Beam w
+ * offers every id i with the score
+ *   d_scores[w] + (logit[w, i] - log sum_j exp(logit[w, j]))   in 64 bits
+ * and the K best (1 .. PZ_BEAM_MAX_SELECT) of a group's W * V, in descending order,
+ * go to d_parent (the beam, 0 .. W - 1), d_ids and d_scores_out (rounded to fp32),
+ * [n_groups, K] each.  Of equal scores the lower beam's comes first, of one beam's
+ * the larger logit's, then the lower id's.  K = W: the next beams; K = 2 W: a choice
+ * from which hypotheses that end leave W that go on.
+ *   d_done [n_groups * W] uint8 or NULL: a beam with a nonzero entry has ended; it
+ *   offers one candidate, pad_id at its score unchanged, and its row is not read.
+ *   d_done_out [n_groups, K] uint8 or NULL: 1 where the parent had ended or the id
+ *   is in the sampler's EOS list (pz_sampler_set_eos).
+ * Logits of -infinity are never chosen.  A beam whose score is not finite, or whose
+ * row has no finite logit, a NaN or +infinity, offers nothing: with d_scores of 0,
+ * -infinity, -infinity, ... a group starts from one hypothesis.  Where fewer than K
+ * are offered the rest reads parent -1, id -1, score -infinity, done 0.  The outputs
+ * must not overlap the inputs.  No limit by the sampler's max_batch or max_vocab.
+ * Asynchronous on the sampler's stream, in a workspace (PZ_BEAM_WORKSPACE bytes)
+ * that the first call allocates; after it, a call can be captured into a HIP graph.
+ * Calls of one sampler, replays included, must be ordered. */
+#define PZ_BEAM_MAX_WIDTH 64
+#define PZ_BEAM_MAX_SELECT 128
+#define PZ_BEAM_WORKSPACE (64 << 20)
+PZ_API int pz_beam_select(pz_sampler *s, const float *d_logits, long ld, int n_groups, int W,
+                          int V, const float *d_scores, const uint8_t *d_done, int32_t pad_id,
+                          int K, int32_t *d_parent, int32_t *d_ids, float *d_scores_out,
+                          uint8_t *d_done_out);
+
+/* Reorders the caches of beams after a selection: beam w of group g becomes a
+ * continuation of beam p = d_parent[g * W + w] of its group.  layers: host array of
+ * n_layers caches (one per layer, read during the call) with the same tables and
+ * lengths, type, shape and pages (d_k and d_v differ); W as pz_beam_select.
+ *   d_len_out [n_groups * W]: the parent's length L.
+ *   d_blocks_out [n_groups * W, max_blocks]: the parent's pages where they are full,
+ *     which its children share.  The page that L ends in (where L is no multiple of
+ *     block_size) stays with the parent's first child; every other child gets a page
+ *     of its own, into which the L % block_size positions are copied, in every
+ *     layer.  Then pages of its own for positions up to L + ahead - 1 (ahead >= 0: how
+ *     many the next step appends; as far as max_blocks goes), then -1.
+ *   d_pool [n_groups, n_pool] (n_pool at most PZ_BEAM_MAX_POOL): the pages that the
+ *     group's beams may own, ascending, of which a page that no beam's table names any
+ *     more is free again: new pages are the lowest free ones, given out in the order
+ *     of beams and positions.  W * max_blocks pages always suffice; tables may also
+ *     name pages outside the pool (a prompt's), which are shared and never given out.
+ *     Groups' pools must not have pages in common.
+ *   d_missing [n_groups] or NULL: how many pages the pool lacked (those entries are
+ *     -1, and what would have been copied is left out), 0 where all is well.
+ * A parent outside [0, W) leaves the beam empty: length 0, a table of -1.  d_blocks_out
+ * and d_len_out must not overlap the caches' own tables and lengths: a program keeps
+ * two of each and takes them in turn.  Asynchronous on the sampler's stream, in
+ * pz_beam_select's workspace (n_groups * W at most PZ_BEAM_MAX_BEAMS); after the first
+ * call of either it can be captured into a HIP graph.  Calls of both on one sampler,
+ * replays included, must be ordered. */
+#define PZ_BEAM_MAX_POOL 262144
+#define PZ_BEAM_MAX_BEAMS (1 << 20)
+PZ_API int pz_beam_reorder(pz_sampler *s, const pz_kv_cache *layers, int n_layers, int n_groups,
+                           int W, const int32_t *d_parent, const int32_t *d_pool, int n_pool,
+                           int ahead, int32_t *d_blocks_out, int32_t *d_len_out,
+                           int32_t *d_missing);
+
 /* Device memory helpers for C hosts (hipMalloc / hipFree / hipMemcpy). */
 PZ_API int pz_device_alloc(void **ptr, size_t bytes, int device);
 PZ_API int pz_device_free(void *ptr);

@@ -1,0 +1,252 @@
+// pz_prefix.hip -- attention of sequences that share prefixes (pz_prefix_attention).
+//
+//   out[r] = sum_p softmax_p(scale q[r] . k[p]) v[p],  p over the positions of the
+//   prefix of r's sequence, its own cached positions and the nodes that r's node sees.
+//
+// The softmax comes in parts that meet at the end, each with its maximum m, its sum l
+// and its sum of values (pz_treedev.h): the prefix's, where the rows of all sequences
+// that share it meet each key, in splits of the longest prefix, and each sequence's
+// own.  k_prefix_join adds them up:
+//   M = max m_i,  out = sum_i 2^(c (m_i - M)) o_i / sum_i 2^(c (m_i - M)) l_i.
+#include <hip/hip_runtime.h>
+
+#include "../../include/pz_sampler.h"
+#include "pz_refuse.h"
+#include "pz_sampler_impl.h"
+#include "pz_treedev.h"
+#include "pz_treeplan.h"
+
+namespace {
+
+// The prefix of the launch's sequence b: -1 where it has none (wave-uniform).
+__device__ __forceinline__ int pf_prefix_of(const SharedArgs& P, int b, int lane) {
+  if (!P.first) return (b + P.b0) / P.each;
+  for (int i0 = 0; i0 < P.B; i0 += 64) {
+    bool it = false;
+    if (i0 + lane < P.B) {
+      int lo;
+      const int n = tr_sharers(P, i0 + lane, &lo);
+      it = lo <= b && b - lo < n;
+    }
+    const uint64_t any = __ballot(it);
+    if (any) return i0 + __ffsll((unsigned long long)any) - 1;
+  }
+  return -1;
+}
+
+// A wave for each head of a node: D / 4 lanes with four results each, 256 / D splits at
+// a time.
+template <int TYPE, int D>
+__global__ __launch_bounds__(256) void k_prefix_join(const OwnArgs A, const SharedArgs P) {
+  constexpr int LANES = D / 4, AT = 64 / LANES;
+  const int lane = threadIdx.x & 63;
+  const int n_heads = A.n_kv * A.group;
+  const size_t row = (size_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (row >= A.R) return;
+  const int node = (int)(row / (unsigned)n_heads), hq = (int)(row - (size_t)node * n_heads);
+  const int b = node / A.T, t = node - b * A.T;
+  if (t >= tr_nodes(A, b)) return;
+  const int i = pf_prefix_of(P, b, lane);
+  int ns = 0;  // splits of the prefix
+  if (i >= 0) {
+    const int chunk = tr_chunk(P, i, lane);
+    ns = (tr_tiles(P, i) + chunk - 1) / chunk;
+  }
+  const int chunk = tr_chunk(A, b, lane), no = (tr_tiles(A, b) + chunk - 1) / chunk;
+  const int at = lane / LANES, d = lane % LANES * 4;
+  float mt = TR_LOW, lt = 0.0f;
+  tr_f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+  auto add = [&](float m, float l, tr_f32x4 v) {
+    const float mn = fmaxf(mt, m), al = tr_lift(mt, mn, A.c), e = tr_lift(m, mn, A.c);
+    mt = mn;
+    lt = lt * al + l * e;
+    o = o * al + v * e;
+  };
+  for (int k = at; k < ns + no; k += AT) {
+    const size_t slot = (size_t)(k < ns ? P.slot + k : A.slot + k - ns) * A.R + row;
+    add(A.ml[2 * slot], A.ml[2 * slot + 1],
+        *reinterpret_cast<const tr_f32x4*>(A.part + slot * D + d));
+  }
+#pragma unroll
+  for (int k = LANES; k < 64; k <<= 1) {
+    const float m = __shfl_xor(mt, k, 64), l = __shfl_xor(lt, k, 64);
+    tr_f32x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = __shfl_xor(o[e], k, 64);
+    add(m, l, v);
+  }
+  // a sum of 0: nothing attended (zeros), or every score -infinity (NaN)
+  float inv = tr_inverse(A, b, t, lt);
+  if (lt == 0.0f && i >= 0) {
+    const int ctx = pz_pages_len(P.pages, P.len[i]);
+    for (int e = 0; (int64_t)e << P.pages.shift < ctx; e++)
+      if ((uint32_t)P.blocks[(size_t)i * P.pages.max_blocks + e] < (uint32_t)P.pages.n_blocks)
+        inv = __builtin_nanf("");
+  }
+  if (at == 0) tr_store4<TYPE>(A.out + (size_t)node * A.ld_out + (size_t)hq * D + d, o * inv);
+}
+
+// Splits of `wgs` workgroups' work of up to `tiles` tiles: a workgroup a CU, and
+// TR_SHARE tiles for each at least.
+int splits(const pz_sampler* s, int64_t wgs, int64_t tiles, int64_t room) {
+  int64_t S = (s->n_cu + wgs - 1) / wgs;
+  S = S < tiles / TR_SHARE ? S : tiles / TR_SHARE;
+  S = S < room ? S : room;
+  S = S < 64 ? S : 64;
+  return (int)(S < 1 ? 1 : S);
+}
+
+template <class ARGS>
+void share_out(ARGS& A, int64_t tiles, int S) {
+  A.chunk = (int)((tiles + S - 1) / S);
+  A.S = (int)((tiles + A.chunk - 1) / A.chunk);
+}
+
+template <int TYPE, int D, int RT, int WAVES>
+void launch_own(pz_sampler* s, OwnArgs& A) {
+  const int64_t groups = ((int64_t)A.B * A.n_kv * A.S + 7) / 8 * 8;
+  hipLaunchKernelGGL((k_tree<TYPE, D, RT, WAVES, OwnArgs>), dim3((unsigned)(groups * A.nblk)),
+                     dim3(64 * WAVES), 0, s->stream, A);
+}
+template <int TYPE, int D, int RT>
+void launch_own_wide(pz_sampler* s, OwnArgs& A) {
+  const int64_t groups = ((int64_t)A.B * A.n_kv * A.S + 7) / 8 * 8;
+  hipLaunchKernelGGL((k_tree_wide<TYPE, D, RT, OwnArgs>),
+                     dim3((unsigned)(groups * (A.nblk / TR_WIDE))), dim3(64 * TR_WIDE), 0,
+                     s->stream, A);
+}
+
+template <int TYPE, int D>
+int run_part(pz_sampler* s, OwnArgs A, SharedArgs P) {
+  const int rows = A.T * A.group;
+  const int64_t most = (int64_t)A.B * rows;  // rows of a key head
+  // (two slots are there: the host takes sequences accordingly)
+  const int64_t slots =
+      (int64_t)(PZ_TREE_WS / ((size_t)(D + 2) * sizeof(float))) / (int64_t)A.R;
+
+  // each sequence's own keys: as pz_tree_attention would take them
+  const int64_t own = ((int64_t)A.pages.max_blocks << A.pages.shift) / TR_KEYS + 1 +
+                      (A.T + TR_KEYS - 1) / TR_KEYS;
+  const int64_t heads = (int64_t)A.B * A.n_kv;
+  const TrKernel kernel = tr_kernel_for(rows, heads, own, s->n_cu, D, A.ld, A.ld_n);
+  const int own_rows = kernel == TR_WIDE32 ? 256 : kernel == TR_WIDE16 ? 128
+                       : kernel == TR_SOME ? 32 : 16;  // of a workgroup
+  const int own_blocks = (rows + own_rows - 1) / own_rows;
+  share_out(A, own, kernel == TR_FEW_SHORT ? 1
+                    : splits(s, heads * own_blocks, own, slots - 1));
+  A.nblk = kernel == TR_WIDE32 || kernel == TR_WIDE16 ? own_blocks * TR_WIDE : own_blocks;
+
+  // the prefixes': the rows of a key head of all who share one
+  const int64_t tiles = ((int64_t)P.pages.max_blocks << P.pages.shift) / TR_KEYS + 1;
+  const TrKernel shared =
+      tr_kernel_for((most + P.B - 1) / P.B, (int64_t)P.B * P.n_kv, tiles, s->n_cu, D, P.ld, 0);
+  const int block = shared == TR_WIDE32 ? 256 : shared == TR_WIDE16 ? 128
+                    : shared == TR_SOME ? 32 : 16;
+  const int64_t blocks = most / block + (P.B < A.B ? P.B : A.B);
+  share_out(P, tiles, splits(s, blocks * P.n_kv, tiles, slots - A.S));
+  if (!pz_launch_fits((blocks * P.n_kv * P.S + 7) / 8 * 8, 512) ||
+      !pz_launch_fits((heads * A.S + 7) / 8 * 8 * A.nblk, 512))
+    return fail(s, PZ_ERANGE, "B=%d sequences of T=%d nodes", A.B, A.T);
+  P.nblk = (int)blocks;
+  P.slot = 0;
+  A.slot = P.S;
+  P.part = A.part = static_cast<float*>(s->tree_dev);
+  P.ml = A.ml = A.part + (size_t)(P.S + A.S) * A.R * D;
+
+  const dim3 grid((unsigned)((blocks * P.n_kv * P.S + 7) / 8 * 8));
+  if (shared == TR_SOME)
+    hipLaunchKernelGGL((k_tree<TYPE, D, 2, 4, SharedArgs>), grid, dim3(256), 0, s->stream, P);
+  else if (shared == TR_FEW || shared == TR_FEW_SHORT)
+    hipLaunchKernelGGL((k_tree<TYPE, D, 1, 4, SharedArgs>), grid, dim3(256), 0, s->stream, P);
+  if (kernel == TR_SOME)
+    launch_own<TYPE, D, 2, 4>(s, A);
+  else if (kernel == TR_FEW || kernel == TR_FEW_SHORT)
+    launch_own<TYPE, D, 1, 4>(s, A);
+  if constexpr (D < 256) {
+    if (shared == TR_WIDE32)
+      hipLaunchKernelGGL((k_tree_wide<TYPE, D, 2, SharedArgs>), grid, dim3(64 * TR_WIDE), 0,
+                         s->stream, P);
+    else if (shared == TR_WIDE16)
+      hipLaunchKernelGGL((k_tree_wide<TYPE, D, 1, SharedArgs>), grid, dim3(64 * TR_WIDE), 0,
+                         s->stream, P);
+    if (kernel == TR_WIDE32)
+      launch_own_wide<TYPE, D, 2>(s, A);
+    else if (kernel == TR_WIDE16)
+      launch_own_wide<TYPE, D, 1>(s, A);
+  }
+  PZ_HIP(s, hipGetLastError());
+  hipLaunchKernelGGL((k_prefix_join<TYPE, D>), dim3((unsigned)((A.R + 3) / 4)), dim3(256), 0,
+                     s->stream, A, P);
+  PZ_HIP(s, hipGetLastError());
+  return PZ_OK;
+}
+
+template <int TYPE>
+int run_type(pz_sampler* s, const OwnArgs& A, const SharedArgs& P, int D) {
+  if (D == 64) return run_part<TYPE, 64>(s, A, P);
+  if (D == 128) return run_part<TYPE, 128>(s, A, P);
+  return run_part<TYPE, 256>(s, A, P);
+}
+
+}  // namespace
+
+extern "C" int pz_prefix_attention(pz_sampler* s, const pz_kv_cache* cache,
+                                   const pz_kv_prefix* prefix, const void* d_kn, const void* d_vn,
+                                   long ld_n, int B, int T, const int32_t* d_n_nodes,
+                                   const uint64_t* d_tree, int n_heads, float scale,
+                                   const void* d_q, long ld_q, void* d_out, long ld_out) {
+  if (!s) return PZ_EINVAL;
+  const PzRefusal no = pz_refuse_prefix(cache, prefix, d_kn, d_vn, ld_n, B, T, n_heads, scale,
+                                        d_q, ld_q, d_out, ld_out);
+  if (no.code) return fail(s, no.code, "%s", no.why);
+  if (B == 0) return PZ_OK;
+  PZ_HIP(s, hipSetDevice(s->device));
+  const int rc = pz_tree_workspace(s);
+  if (rc != PZ_OK) return rc;
+  const int D = cache->head_dim;
+  const int shift = __builtin_ctz((unsigned)cache->block_size);
+  const size_t per = (size_t)T * n_heads;  // results of a sequence in a slot
+  // as many sequences at a time as two slots hold
+  int64_t step = (int64_t)(PZ_TREE_WS / (2 * (size_t)(D + 2) * sizeof(float)) / per);
+  step = step < B ? step : B;
+  for (int b0 = 0; b0 < B; b0 += (int)step) {
+    const int nb = B - b0 < step ? B - b0 : (int)step;
+    const size_t node0 = (size_t)b0 * T;
+    OwnArgs A = {};
+    A.k = static_cast<const uint16_t*>(cache->d_k);
+    A.v = static_cast<const uint16_t*>(cache->d_v);
+    A.ld = cache->ld;
+    A.T = T;
+    A.n_kv = cache->n_kv_heads;
+    A.group = n_heads / cache->n_kv_heads;
+    A.c = scale * TR_LOG2E;
+    A.q = static_cast<const uint16_t*>(d_q) + node0 * ld_q;
+    A.ld_q = ld_q;
+    A.out = static_cast<uint16_t*>(d_out) + node0 * ld_out;
+    A.ld_out = ld_out;
+    A.R = (size_t)nb * per;
+    SharedArgs P = {};
+    static_cast<PartArgs&>(P) = A;
+    P.B = prefix->n_prefixes;
+    P.pages = {cache->n_blocks, shift, prefix->max_blocks};
+    P.blocks = prefix->d_blocks;
+    P.len = prefix->d_len;
+    P.first = prefix->d_first;
+    P.each = B / prefix->n_prefixes;
+    P.b0 = b0;
+    P.nb = nb;
+    A.B = nb;
+    A.pages = {cache->n_blocks, shift, cache->max_blocks};
+    A.blocks = cache->d_blocks + (size_t)b0 * cache->max_blocks;
+    A.len = cache->d_len + b0;
+    A.kn = static_cast<const uint16_t*>(d_kn) + node0 * ld_n;
+    A.vn = static_cast<const uint16_t*>(d_vn) + node0 * ld_n;
+    A.ld_n = ld_n;
+    A.n_nodes = d_n_nodes ? d_n_nodes + b0 : nullptr;
+    A.tree = d_tree ? d_tree + node0 : nullptr;
+    const int rc = cache->type == PZ_BF16 ? run_type<PZ_BF16>(s, A, P, D)
+                                          : run_type<PZ_F16>(s, A, P, D);
+    if (rc != PZ_OK) return rc;
+  }
+  return PZ_OK;
+}

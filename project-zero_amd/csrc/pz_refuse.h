@@ -1,6 +1,6 @@
-// pz_refuse.h -- which calls of the logit rules, the 8-bit LM head and the
-// tree attention are refused, and why.  Host only and without a device, so
-// that the refusals have a test of their own.
+// pz_refuse.h -- which calls of the logit rules, the 8-bit LM head, the attention
+// over a paged cache and the beam search are refused, and why.  Host only and
+// without a device, so that the refusals have a test of their own.
 #pragma once
 #include <stddef.h>
 #include <stdint.h>
@@ -13,6 +13,10 @@ struct PzRefusal {
 };
 constexpr int PZ_MOST = 1 << 30;  // of ids and list entries, so that 32-bit counters can step past
 constexpr int PZ_MOST_HEADS = 1 << 16;  // so that rows and row lengths fit 32 bits
+constexpr int PZ_MOST_PREFIXES = 1 << 20;
+constexpr int PZ_MOST_ROWS = 1 << 15;  // of a sequence in prefix attention, so that its
+                                       // results of two parts fit the workspace
+constexpr int PZ_MOST_IDS = 1 << 22;   // of a selection, whose lists of one row are in the workspace
 constexpr PzRefusal PZ_TAKEN = {PZ_OK, nullptr};
 
 // Whether a launch of `wgs` workgroups fits: their threads have 32-bit numbers.
@@ -103,5 +107,106 @@ inline PzRefusal pz_refuse_tree(const pz_kv_cache* c, const void* d_kn, const vo
   if (!d_q || !d_out || ld_q < row || ld_out < row) return {PZ_EINVAL, "bad q or out"};
   if (ld_q % 8 || ld_out % 8 || !pz_aligned16(d_q) || !pz_aligned16(d_out))
     return {PZ_EINVAL, "strides are multiples of 8, pointers 16-byte aligned"};
+  return PZ_TAKEN;
+}
+
+inline PzRefusal pz_refuse_prefix(const pz_kv_cache* c, const pz_kv_prefix* p, const void* d_kn,
+                                  const void* d_vn, long ld_n, int B, int T, int n_heads,
+                                  float scale, const void* d_q, long ld_q, const void* d_out,
+                                  long ld_out) {
+  const PzRefusal r =
+      pz_refuse_tree(c, d_kn, d_vn, ld_n, B, T, n_heads, scale, d_q, ld_q, d_out, ld_out);
+  if (r.code) return r;
+  if (!p || !p->d_blocks || !p->d_len || p->max_blocks <= 0 || p->n_prefixes <= 0)
+    return {PZ_EINVAL, "bad prefix"};
+  if ((int64_t)p->max_blocks * c->block_size > INT32_MAX - 64)
+    return {PZ_ERANGE, "the prefix's max_blocks * block_size does not fit 32 bits"};
+  if (!p->d_first && B % p->n_prefixes)
+    return {PZ_EINVAL, "without d_first n_prefixes divides B"};
+  if (p->n_prefixes > PZ_MOST_PREFIXES) return {PZ_ERANGE, "n_prefixes above 2^20"};
+  if ((int64_t)T * n_heads > PZ_MOST_ROWS) return {PZ_ERANGE, "T * n_heads above 32768"};
+  return PZ_TAKEN;
+}
+
+inline PzRefusal pz_refuse_rope(const pz_qk_rope* r, const void* d_q, long ld_q, const void* d_k,
+                                long ld_k, const void* d_qo, long ld_qo, const void* d_ko,
+                                long ld_ko, int n, const int32_t* d_pos) {
+  if (!r || n < 0 || r->n_heads < 0 || r->n_kv_heads < 0 || r->n_heads + r->n_kv_heads <= 0)
+    return {PZ_EINVAL, "bad heads or tokens"};
+  if (r->type != PZ_F32 && r->type != PZ_BF16 && r->type != PZ_F16)
+    return {PZ_EINVAL, "type is PZ_F32, PZ_BF16 or PZ_F16"};
+  if (r->head_dim <= 0) return {PZ_EINVAL, "bad head_dim"};
+  if (r->head_dim > 1024) return {PZ_ENOTSUP, "head_dim above 1024"};
+  if (r->n_heads > PZ_MOST_HEADS || r->n_kv_heads > PZ_MOST_HEADS)
+    return {PZ_ERANGE, "n_heads or n_kv_heads above 65536"};
+  if (r->rot_dim < 0 || r->rot_dim > r->head_dim || r->rot_dim % 2)
+    return {PZ_EINVAL, "rot_dim is even, 0 to head_dim"};
+  if (r->layout != PZ_ROPE_HALVES && r->layout != PZ_ROPE_PAIRS)
+    return {PZ_EINVAL, "layout is PZ_ROPE_HALVES or PZ_ROPE_PAIRS"};
+  if (r->rot_dim && (!r->d_freq || !d_pos)) return {PZ_EINVAL, "a rotation needs d_freq and d_pos"};
+  if ((r->d_q_norm || r->d_k_norm) && !(r->eps >= 0.0f && r->eps < 3.0e38f))
+    return {PZ_EINVAL, "eps is finite and not negative"};
+  const uintptr_t odd = r->type == PZ_F32 ? 3 : 1;
+  const struct {
+    const void *in, *out;
+    long ld_in, ld_out;
+    int heads;
+  } parts[2] = {{d_q, d_qo, ld_q, ld_qo, r->n_heads}, {d_k, d_ko, ld_k, ld_ko, r->n_kv_heads}};
+  for (const auto& p : parts) {
+    if (!p.heads) continue;
+    const long row = (long)p.heads * r->head_dim;
+    if (!p.in || !p.out || p.ld_in < row || p.ld_out < row)
+      return {PZ_EINVAL, "bad rows: null, or a stride less than heads * head_dim"};
+    if (p.in == p.out && p.ld_in != p.ld_out) return {PZ_EINVAL, "in place needs equal strides"};
+    if (((uintptr_t)p.in & odd) || ((uintptr_t)p.out & odd))
+      return {PZ_EINVAL, "rows are not aligned to their type"};
+  }
+  if (((uintptr_t)r->d_q_norm | (uintptr_t)r->d_k_norm | (uintptr_t)r->d_freq) & 3)
+    return {PZ_EINVAL, "d_q_norm, d_k_norm or d_freq is not aligned to 4 bytes"};
+  // (a wave for every head is the most that a launch takes)
+  if (!pz_launch_fits((int64_t)n * (r->n_heads + r->n_kv_heads), 64))
+    return {PZ_ERANGE, "more tokens and heads than a launch takes"};
+  return PZ_TAKEN;
+}
+
+inline PzRefusal pz_refuse_select(const float* d_logits, long ld, int n_groups, int W, int V,
+                                  const float* d_scores, int K, const int32_t* d_parent,
+                                  const int32_t* d_ids, const float* d_scores_out) {
+  if (!d_logits || !d_scores || !d_parent || !d_ids || !d_scores_out || n_groups < 0 || V <= 0 ||
+      ld < V)
+    return {PZ_EINVAL, "bad logits, scores or outputs"};
+  if (W <= 0 || K <= 0) return {PZ_EINVAL, "W and K are positive"};
+  if (W > PZ_BEAM_MAX_WIDTH) return {PZ_ERANGE, "W > PZ_BEAM_MAX_WIDTH"};
+  if (K > PZ_BEAM_MAX_SELECT) return {PZ_ERANGE, "K > PZ_BEAM_MAX_SELECT"};
+  if (V > PZ_MOST_IDS) return {PZ_ERANGE, "V above 2^22"};
+  if (n_groups > PZ_BEAM_MAX_BEAMS) return {PZ_ERANGE, "n_groups above 2^20"};
+  return PZ_TAKEN;
+}
+
+inline PzRefusal pz_refuse_reorder(const pz_kv_cache* layers, int n_layers, int n_groups, int W,
+                                   const int32_t* d_parent, const int32_t* d_pool, int n_pool,
+                                   int ahead, const int32_t* d_blocks_out,
+                                   const int32_t* d_len_out) {
+  if (!layers || n_layers <= 0 || n_groups < 0 || !d_parent || !d_blocks_out || !d_len_out)
+    return {PZ_EINVAL, "bad layers, parents or outputs"};
+  if (W <= 0) return {PZ_EINVAL, "W is positive"};
+  if (W > PZ_BEAM_MAX_WIDTH) return {PZ_ERANGE, "W > PZ_BEAM_MAX_WIDTH"};
+  if (n_pool < 0 || (n_pool > 0 && !d_pool)) return {PZ_EINVAL, "n_pool>0 needs d_pool"};
+  if (n_pool > PZ_BEAM_MAX_POOL) return {PZ_ERANGE, "n_pool > PZ_BEAM_MAX_POOL"};
+  if (ahead < 0) return {PZ_EINVAL, "ahead is not negative"};
+  if ((int64_t)n_groups * W > PZ_BEAM_MAX_BEAMS)
+    return {PZ_ERANGE, "n_groups * W > PZ_BEAM_MAX_BEAMS"};
+  for (int i = 0; i < n_layers; i++) {
+    const pz_kv_cache &c = layers[i], &o = layers[0];
+    const PzRefusal r = pz_refuse_cache(&c, c.d_k, c.d_v, c.ld, n_groups * W, 1);
+    if (r.code) return r;
+    if (c.type != o.type || c.n_kv_heads != o.n_kv_heads || c.head_dim != o.head_dim ||
+        c.ld != o.ld || c.n_blocks != o.n_blocks || c.block_size != o.block_size ||
+        c.d_blocks != o.d_blocks || c.max_blocks != o.max_blocks || c.d_len != o.d_len)
+      return {PZ_EINVAL, "layers differ in more than d_k and d_v"};
+  }
+  if ((int64_t)W * layers[0].max_blocks > PZ_MOST) return {PZ_ERANGE, "W * max_blocks above 2^30"};
+  if (d_blocks_out == layers[0].d_blocks || d_len_out == layers[0].d_len)
+    return {PZ_EINVAL, "new tables and lengths are not the old ones"};
   return PZ_TAKEN;
 }

@@ -62,9 +62,12 @@ struct pz_sampler {
   uint16_t* d_lmh_x = nullptr;
   size_t lmh_x_elems = 0;
 
-  // tree attention's partial results (PZ_TREE_WS bytes, allocated by its first
-  // call and kept, so captured calls stay valid)
+  // partial results of tree and prefix attention (PZ_TREE_WS bytes, allocated by the
+  // first call and kept, so captured calls stay valid)
   void* tree_dev = nullptr;
+  // candidates of a beam selection, copies of a reordering (PZ_BEAM_WORKSPACE bytes,
+  // alike)
+  void* beam_dev = nullptr;
 
   const float* call_u = nullptr;  // the synchronous call's host uniforms, during the call
 
@@ -152,6 +155,9 @@ int pz_launch_softmax_rows(pz_sampler* s, const float* d_in, long ld_in, float* 
 int pz_launch_softmax_split(pz_sampler* s, const PzSplitWs& ws, const float* d_in, long ld_in,
                             float* d_out, long ld_out, int n_rows, int n, PzTemp T,
                             const int32_t* d_len);
+
+// The attention workspace s->tree_dev, allocated by the first call.
+int pz_tree_workspace(pz_sampler* s);
 
 // Ids from the fused LM heads' argmax keys (s->d_lmh_keys, s->d_lmh_nan),
 // which it clears for the next call.

@@ -20,6 +20,9 @@ PZ_TEMP_MUL_RECIP, PZ_TEMP_DIV = 0, 1
 PZ_F32, PZ_BF16, PZ_F16 = 0, 1, 2
 PZ_I8_MAX_N = 131071
 PZ_TREE_MAX_NODES = 64
+PZ_ROPE_HALVES, PZ_ROPE_PAIRS = 0, 1
+PZ_BEAM_MAX_WIDTH, PZ_BEAM_MAX_SELECT = 64, 128
+PZ_BEAM_WORKSPACE, PZ_BEAM_MAX_POOL, PZ_BEAM_MAX_BEAMS = 64 << 20, 262144, 1 << 20
 
 # Every symbol include/pz_sampler.h and include/pz_sampling_compat.h declare.
 ABI_SYMBOLS = (
@@ -32,7 +35,8 @@ ABI_SYMBOLS = (
     "pz_lm_head_argmax_bf16", "pz_spec_decode", "pz_sampler_set_wait_bound",
     "pz_spec_verify_greedy", "pz_spec_verify_greedy_async", "pz_spec_decode_opts",
     "pz_rules_batch", "pz_quant_rows_i8", "pz_lm_head_i8", "pz_lm_head_argmax_i8",
-    "pz_tree_attention", "pz_cache_append",
+    "pz_tree_attention", "pz_cache_append", "pz_prefix_attention", "pz_qk_norm_rope",
+    "pz_beam_select", "pz_beam_reorder",
     # include/pz_sampling_compat.h: the reference sampler's own symbols
     "sample_argmax", "apply_temperature", "sample_top_p", "sample_top_k", "rng_seed",
     "rng_float", "pz_tn_softmax", "pz_compat_set_temp_mode", "pz_compat_last_status",
@@ -98,6 +102,32 @@ class KvCache(ctypes.Structure):
     ]
 
 
+class KvPrefix(ctypes.Structure):
+    _fields_ = [
+        ("d_blocks", ctypes.c_void_p),
+        ("max_blocks", ctypes.c_int),
+        ("d_len", ctypes.c_void_p),
+        ("n_prefixes", ctypes.c_int),
+        ("d_first", ctypes.c_void_p),
+    ]
+
+
+class QkRope(ctypes.Structure):
+    _fields_ = [
+        ("type", ctypes.c_int),
+        ("n_heads", ctypes.c_int),
+        ("n_kv_heads", ctypes.c_int),
+        ("head_dim", ctypes.c_int),
+        ("d_q_norm", ctypes.c_void_p),
+        ("d_k_norm", ctypes.c_void_p),
+        ("eps", ctypes.c_float),
+        ("rot_dim", ctypes.c_int),
+        ("layout", ctypes.c_int),
+        ("d_freq", ctypes.c_void_p),
+        ("amplitude", ctypes.c_float),
+    ]
+
+
 def _filled(struct, kw):
     """struct with its device buffers (d_*) by address; it keeps them alive."""
     names = {n for n, _ in struct._fields_}
@@ -119,6 +149,16 @@ def logit_rules(rep_penalty=1.0, presence_penalty=0.0, frequency_penalty=0.0, **
 def kv_cache(**kw):
     """pz_kv_cache; device buffers as addresses or torch tensors."""
     return _filled(KvCache, kw)
+
+
+def kv_prefix(**kw):
+    """pz_kv_prefix; device buffers as addresses or torch tensors."""
+    return _filled(KvPrefix, kw)
+
+
+def qk_rope(eps=1e-6, layout=PZ_ROPE_HALVES, amplitude=1.0, **kw):
+    """pz_qk_rope; device buffers as addresses or torch tensors."""
+    return _filled(QkRope, dict(kw, eps=eps, layout=layout, amplitude=amplitude))
 
 
 _lib = None
@@ -181,6 +221,14 @@ def load():
     lib.pz_tree_attention.argtypes = [_P, ctypes.POINTER(KvCache), _P, _P, _L, _I, _I, _P, _P, _I,
                                       _F, _P, _L, _P, _L]
     lib.pz_cache_append.argtypes = [_P, ctypes.POINTER(KvCache), _P, _P, _L, _I, _I, _P, _P]
+    lib.pz_prefix_attention.argtypes = [_P, ctypes.POINTER(KvCache), ctypes.POINTER(KvPrefix), _P,
+                                        _P, _L, _I, _I, _P, _P, _I, _F, _P, _L, _P, _L]
+    lib.pz_qk_norm_rope.argtypes = [_P, ctypes.POINTER(QkRope), _P, _L, _P, _L, _P, _L, _P, _L, _I,
+                                    _P]
+    lib.pz_beam_select.argtypes = [_P, _P, _L, _I, _I, _I, _P, _P, ctypes.c_int32, _I, _P, _P, _P,
+                                   _P]
+    lib.pz_beam_reorder.argtypes = [_P, ctypes.POINTER(KvCache), _I, _I, _I, _P, _P, _I, _I, _P,
+                                    _P, _P]
     pull = ctypes.POINTER(ctypes.c_ulonglong)
     lib.sample_argmax.argtypes = [_P, _I]
     lib.apply_temperature.argtypes = [_P, _I, _F]
@@ -417,6 +465,42 @@ class Sampler:
         _sync_torch(d_kn, d_vn, *getattr(cache, "buffers", ()))
         self._check(self.lib.pz_cache_append(self.h, ctypes.byref(cache), _ptr(d_kn), _ptr(d_vn),
                                              ld_n, B, T, _ptr(d_take), _ptr(d_count)))
+
+    def prefix_attention(self, cache, prefix, d_kn, d_vn, ld_n, B, T, n_heads, scale, d_q, ld_q,
+                         d_out, ld_out, d_n_nodes=None, d_tree=None):
+        """tree_attention with kv_prefix(...) before the sequences' own positions
+        (asynchronous)."""
+        _sync_torch(d_q, d_kn, d_out, *getattr(cache, "buffers", ()))
+        self._check(self.lib.pz_prefix_attention(
+            self.h, ctypes.byref(cache), ctypes.byref(prefix), _ptr(d_kn), _ptr(d_vn), ld_n, B, T,
+            _ptr(d_n_nodes), _ptr(d_tree), n_heads, scale, _ptr(d_q), ld_q, _ptr(d_out), ld_out))
+
+    def qk_norm_rope(self, rope, d_q, ld_q, d_k, ld_k, d_q_out, ld_q_out, d_k_out, ld_k_out, n,
+                     d_pos):
+        """Norms of the heads of n tokens' queries and keys and their rotation,
+        qk_rope(...) (asynchronous)."""
+        _sync_torch(d_q, d_k, d_q_out, d_k_out, d_pos, *getattr(rope, "buffers", ()))
+        self._check(self.lib.pz_qk_norm_rope(
+            self.h, ctypes.byref(rope), _ptr(d_q), ld_q, _ptr(d_k), ld_k, _ptr(d_q_out), ld_q_out,
+            _ptr(d_k_out), ld_k_out, n, _ptr(d_pos)))
+
+    def beam_select(self, d_logits, ld, n_groups, W, V, d_scores, K, d_parent, d_ids,
+                    d_scores_out, d_done=None, pad_id=0, d_done_out=None):
+        """The K best continuations of each group's W beams (asynchronous)."""
+        _sync_torch(d_logits, d_scores, d_done, d_parent, d_ids, d_scores_out, d_done_out)
+        self._check(self.lib.pz_beam_select(
+            self.h, _ptr(d_logits), ld, n_groups, W, V, _ptr(d_scores), _ptr(d_done), pad_id, K,
+            _ptr(d_parent), _ptr(d_ids), _ptr(d_scores_out), _ptr(d_done_out)))
+
+    def beam_reorder(self, layers, n_groups, W, d_parent, d_pool, n_pool, ahead, d_blocks_out,
+                     d_len_out, d_missing=None):
+        """The chosen beams' tables, lengths and pages in every layer's kv_cache(...)
+        (asynchronous)."""
+        _sync_torch(d_parent, d_pool, *(b for c in layers for b in getattr(c, "buffers", ())))
+        arr = (KvCache * len(layers))(*layers)
+        self._check(self.lib.pz_beam_reorder(
+            self.h, arr, len(layers), n_groups, W, _ptr(d_parent), _ptr(d_pool), n_pool, ahead,
+            _ptr(d_blocks_out), _ptr(d_len_out), _ptr(d_missing)))
 
     def spec_verify(self, d_target, d_draft, B, K, V, ld, has_bonus, temperature,
                     draft_ids, u_acc, u_res):
