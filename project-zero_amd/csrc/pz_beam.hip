@@ -3,19 +3,23 @@
 //
 // Selection.  score[w, i] = d_scores[w] + (x[w, i] - lse_w), lse_w = log sum_j exp(x[w, j]).
 // Beams of a group lie close together, so that lse decides between their candidates: it is
-// held in 64 bits.  Its exponentials come from the series of exp on [-ln 2 / 2, ln 2 / 2],
-// whose terms past x^11 are below 2^-47; a 64-bit fma takes a wave as long as a 32-bit one
-// here, and a row's read hides them.  Within a beam the score rises with the logit, so that
-// a row's K best are the K largest logits:
+// held in 64 bits, its exponentials to 2^-43.  (A 64-bit fma takes a wave as long as a
+// 32-bit one here.)  Within a beam the score rises with the logit, so that a row's K best
+// are the K largest logits:
 //
 //   * k_beam_row: a workgroup a segment of a row, which it reads once, to registers:
 //     maximum, sum of exponentials, and its K best as keys (order key of the logit, then
-//     the id counted down: larger is better).  Of the threads' maxima the K-th largest,
-//     found by its leading digits, is a bound that K elements reach; the few above it meet
-//     in LDS, where each counts those that are better.
+//     the id counted down: larger is better).  The threads' maxima meet in groups, the K-th
+//     largest of which is a bound that K elements reach; the few at or above it meet in
+//     LDS, where each counts those that are better.
 //   * k_beam_join: a workgroup a group; the same over its beams' candidates.
 //
-// Where more elements tie at the bound than LDS has room for, the K best are taken one by one.
+// Where more elements tie at the bound than LDS has room for, the K best are taken one by
+// one.  Bound by the read of the logits with the vector instructions (13 an id) close
+// behind: 256 rows of 151936 ids (10% ended, 140 MB) 35 us, 4.0 TB/s, and 6 to join; 47
+// us with a series of 12 terms in place of the table.  Few rows take segments of 2048
+// ids, so that they fill the CUs (8 rows of 128256 ids: 12 us); of 8192 otherwise (64 rows
+// 26 us, 38 in 2048).
 #include <hip/hip_runtime.h>
 
 #include "../../include/pz_sampler.h"
@@ -28,18 +32,17 @@ namespace {
 
 constexpr int BE_CAP = 2048;   // elements of a segment that meet in LDS
 constexpr int BE_JCAP = 1024;  // candidates of a group that do
-constexpr int BE_SLACK = 64;   // how many more than K a bound may let through
 
 struct BeamStat {
-  double sum;  // of exp(x - m)
+  double sum;  // of exp(x - m); not finite where a logit is NaN or +infinity
   float m;     // the segment's maximum, -infinity without a finite logit
-  int bad;     // a NaN or +infinity
 };
 
 struct BeamArgs {
   const float* x;
   long ld;
   int W, V, S, K;  // beams, ids, segments of a row
+  float per_list, per_segment;  // 1 / (W S), 1 / S
   const float* score;
   const uint8_t* done;
   int32_t pad;
@@ -53,24 +56,46 @@ struct BeamArgs {
   int n_eos;
 };
 
-// exp(d), d <= 0.
-__device__ __forceinline__ double be_exp(double d) {
-  d = d > -1000.0 ? d : -1000.0;  // (0 from -746 on)
-  const double t = d * 1.44269504088896340736, k = rint(t);
-  const double r = (t - k) * 0.69314718055994530942;
-  double p = 1.0 / 39916800.0;
-  p = __builtin_fma(r, p, 1.0 / 3628800.0);
-  p = __builtin_fma(r, p, 1.0 / 362880.0);
-  p = __builtin_fma(r, p, 1.0 / 40320.0);
-  p = __builtin_fma(r, p, 1.0 / 5040.0);
-  p = __builtin_fma(r, p, 1.0 / 720.0);
-  p = __builtin_fma(r, p, 1.0 / 120.0);
-  p = __builtin_fma(r, p, 1.0 / 24.0);
-  p = __builtin_fma(r, p, 1.0 / 6.0);
+// exp(x) = 2^(n / 32) exp(r), n the whole number nearest to 32 x / ln 2 (which the sum with
+// 1.5 2^52 leaves in its last bits) and |r| <= ln 2 / 64: 2^(n % 32 / 32) from a table, n / 32
+// into its exponent, and exp(r) from its series up to r^4, with r^5 / 120 replaced by
+// the cubic that is nearest on the interval (Chebyshev's): 2^-43 is left.
+// (The table: the bits of 2^(i / 32) less i 2^47, so that all of n may be added.)
+__constant__ const uint64_t be_roots[32] = {
+    0x3ff0000000000000ull, 0x3fefd9b0d3158574ull, 0x3fefb5586cf9890full, 0x3fef9301d0125b51ull,
+    0x3fef72b83c7d517bull, 0x3fef54873168b9aaull, 0x3fef387a6e756238ull, 0x3fef1e9df51fdee1ull,
+    0x3fef06fe0a31b715ull, 0x3feef1a7373aa9cbull, 0x3feedea64c123422ull, 0x3feece086061892dull,
+    0x3feebfdad5362a27ull, 0x3feeb42b569d4f82ull, 0x3feeab07dd485429ull, 0x3feea47eb03a5585ull,
+    0x3feea09e667f3bcdull, 0x3fee9f75e8ec5f74ull, 0x3feea11473eb0187ull, 0x3feea589994cce13ull,
+    0x3feeace5422aa0dbull, 0x3feeb737b0cdc5e5ull, 0x3feec49182a3f090ull, 0x3feed503b23e255dull,
+    0x3feee89f995ad3adull, 0x3feeff76f2fb5e47ull, 0x3fef199bdd85529cull, 0x3fef3720dcef9069ull,
+    0x3fef5818dcfba487ull, 0x3fef7c97337b9b5full, 0x3fefa4afa2a490daull, 0x3fefd0765b6e4540ull};
+constexpr double BE_PER = 46.1662413084468290355, BE_STEP = 0.0216608493924982909193;
+constexpr double BE_C1 = 0.999999999964169676946, BE_C3 = 0.166667888521865636702;
+constexpr float BE_PLAIN = 500.0f;  // largest |m| whose exponentials are taken as they are
+constexpr float BE_LEAST = -650.0f;  // smaller logits count as this beside such an m (10^-65 of it)
+typedef uint32_t be_u32x2 __attribute__((ext_vector_type(2)));  // low, high
+typedef __attribute__((address_space(3))) const be_u32x2* be_table;
+__device__ __forceinline__ be_u32x2 be_bits(uint64_t v) { return __builtin_bit_cast(be_u32x2, v); }
+// sum + exp(d), |d| <= 700
+__device__ __forceinline__ double be_add_exp(double sum, double d, be_table roots) {
+  constexpr double ROUND = 6755399441055744.0;  // 1.5 2^52
+  const double t = __builtin_fma(d, BE_PER, ROUND), n = t - ROUND;
+  const double r = __builtin_fma(n, -BE_STEP, d);
+  const uint32_t k = (uint32_t)__builtin_bit_cast(uint64_t, t);
+  be_u32x2 root = roots[k & 31u];
+  root[1] += k << 15;
+  const double scale = __builtin_bit_cast(double, root);
+  double p = __builtin_fma(r, 1.0 / 24.0, BE_C3);
   p = __builtin_fma(r, p, 0.5);
+  p = __builtin_fma(r, p, BE_C1);
   p = __builtin_fma(r, p, 1.0);
-  p = __builtin_fma(r, p, 1.0);
-  return __builtin_ldexp(p, (int)k);
+  return __builtin_fma(p, scale, sum);
+}
+// exp(x - m), x <= m
+__device__ __forceinline__ double be_exp(float x, float m, be_table roots) {
+  const double d = (double)x - (double)m;
+  return be_add_exp(0.0, d < -700.0 ? -700.0 : d, roots);  // (10^-304 at least; a NaN stays)
 }
 
 __device__ __forceinline__ double be_wave_sum(double v) {
@@ -84,63 +109,87 @@ __device__ __forceinline__ uint64_t be_key(float x, int id) {
 }
 constexpr uint32_t BE_NONE = 0x007fffffu;  // the order key of -infinity
 
-// The bound T of at most 32 leading bits that at least K of the keys reach (0 where there
-// are fewer), found digit by digit until it lets no more than K + BE_SLACK of them through.
-// each(f) calls f(key) for this thread's keys; keys of 0 are none.  hist: LDS [256].
-template <int BLOCK, class EACH>
-__device__ __forceinline__ uint32_t be_bound(int K, uint32_t* hist, EACH each) {
-  const int lane = threadIdx.x & 63;
-  uint32_t T = 0u;
-  int need = K;  // of the keys that share T's digits so far
-  for (int sh = 24; sh >= 0; sh -= 8) {
-    for (int i = threadIdx.x; i < 256; i += BLOCK) hist[i] = 0u;
-    __syncthreads();
-    each([&](uint32_t key) {
-      if (key && (sh == 24 || key >> (sh + 8) == T >> (sh + 8)))
-        atomicAdd(&hist[key >> sh & 255u], 1u);
-    });
-    __syncthreads();
-    // (every wave for itself) lane l's four digits, and how many keys lie above
-    uint32_t n[4], own = 0u;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      n[i] = hist[4 * lane + i];
-      own += n[i];
+// max(v, v of the lane that DPP control CTRL names), CTRL one that gives every lane one.
+template <int CTRL>
+__device__ __forceinline__ float be_max_dpp(float v) {
+  return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf,
+                                                             true)));
+}
+template <int CTRL>
+__device__ __forceinline__ double be_max_dpp(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t l = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xf, 0xf, true),
+                 h = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, 0xf, 0xf, true);
+  return fmax(v, __builtin_bit_cast(double, (uint64_t)h << 32 | l));
+}
+
+// A bound that at least K of the block's elements reach, -infinity where there are fewer:
+// the K-th largest of the maxima of groups of threads (64, 16, 4 or 2 each, while there are
+// 2 K of these at least, else 1; at least K).  mine: the thread's largest (-infinity
+// without one); *most: the block's.  lds: BLOCK + 1 numbers.  One barrier, two with more
+// than 64 groups, of which each wave then looks at 64 (all of them in every wave: one beam
+// of 128256 ids, the 128 best: 92 us, 45 so).
+template <int BLOCK, class F>
+__device__ __forceinline__ F be_bound(F mine, int K, F* lds, F* most) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  int shift = 0;  // of a group's threads
+  if (BLOCK / 2 >= 2 * K) {
+    mine = be_max_dpp<0xb1>(mine);  // the neighbour
+    shift = 1;
+    if (BLOCK / 4 >= 2 * K) {
+      mine = be_max_dpp<0x4e>(mine);  // the other pair of a quad
+      shift = 2;
     }
-    uint32_t sum = own;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint32_t v = __shfl_down(sum, o, 64);
-      sum += lane + o < 64 ? v : 0u;
+    if (BLOCK / 16 >= 2 * K) {
+      mine = be_max_dpp<0x141>(mine);  // the eight mirrored, then the row's sixteen
+      mine = be_max_dpp<0x140>(mine);
+      shift = 4;
     }
-    const uint64_t enough = __ballot((int)sum >= need);
-    __syncthreads();  // (hist is cleared next)
-    if (!enough) return 0u;  // (only at the first digit)
-    const int at = 63 - __clzll((unsigned long long)enough);
-    int above = (int)(sum - own), digit = 3;
-#pragma unroll
-    for (int i = 3; i > 0; i--)
-      if (digit == i && above + (int)n[i] < need) {
-        above += (int)n[i];
-        digit = i - 1;
-      }
-    const uint32_t in = digit == 3 ? n[3] : digit == 2 ? n[2] : digit == 1 ? n[1] : n[0];
-    const int d = __builtin_amdgcn_readlane(4 * lane + digit, at);
-    need -= __builtin_amdgcn_readlane(above, at);
-    T |= (uint32_t)d << sh;
-    if (__builtin_amdgcn_readlane((int)in, at) - need <= BE_SLACK) break;
+    if (BLOCK / 64 >= 2 * K) {
+      F v = __shfl_xor(mine, 16, 64);
+      mine = v > mine ? v : mine;
+      v = __shfl_xor(mine, 32, 64);
+      mine = v > mine ? v : mine;
+      shift = 6;
+    }
   }
-  return T;
+  const int groups = BLOCK >> shift;
+  if ((tid & ((1 << shift) - 1)) == 0) lds[tid >> shift] = mine;
+  if (tid == 0) lds[BLOCK] = -__builtin_inff();
+  pz_lds_barrier();
+  const int at = (groups > 64 ? tid & ~63 : 0) + lane;
+  const bool on = at < groups;
+  const F v = lds[on ? at : 0];
+  F top = -__builtin_inff(), bound = -__builtin_inff();
+  int more = 0, least = 0;  // groups above it, groups that it does not pass
+  // (a multiple of four; no short cuts, which would be branches and a wait for each number)
+#pragma unroll 4
+  for (int j = 0; j < groups; j++) {
+    const F o = lds[j];
+    more += o > v;
+    least += o >= v;
+    top = o > top ? o : top;
+  }
+  const bool is = on & (more < K) & (least >= K);  // (equal ones together)
+  const uint64_t kth = __ballot(is);
+  if (groups > 64) {
+    if (is) lds[BLOCK] = v;
+    pz_lds_barrier();
+    bound = lds[BLOCK];
+  } else if (kth) {
+    bound = __shfl(v, __ffsll((unsigned long long)kth) - 1, 64);
+  }
+  *most = top;
+  return bound;
 }
 
 template <int BLOCK, int NV>
-__global__ __launch_bounds__(BLOCK) void k_beam_row(const BeamArgs A) {
+__global__ __launch_bounds__(BLOCK) __attribute__((amdgpu_waves_per_eu(6, 8))) void k_beam_row(const BeamArgs A) {
   constexpr int WAVES = BLOCK / 64, N = 4 * NV;
-  __shared__ uint64_t list[BE_CAP];
-  __shared__ uint32_t hist[256];
+  __shared__ uint64_t list[BE_CAP + 8];
   __shared__ double part[WAVES];
-  __shared__ float top[WAVES];
-  __shared__ int flag[WAVES];
+  __shared__ be_u32x2 roots[32];
+  __shared__ float tops[BLOCK + 1];
   __shared__ int n_list;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int row = blockIdx.x / A.S, seg = blockIdx.x - row * A.S;
@@ -150,78 +199,85 @@ __global__ __launch_bounds__(BLOCK) void k_beam_row(const BeamArgs A) {
   const float* x = A.x + (size_t)row * A.ld;
   const int base = seg * (BLOCK * N);
   float v[N];
+  if (base + BLOCK * N <= A.V) {
 #pragma unroll
-  for (int j = 0; j < NV; j++) {
-    const int i = base + (j * BLOCK + tid) * 4;
-    if (i + 3 < A.V) {
-      const pz_f4u q = *reinterpret_cast<const pz_f4u*>(x + i);
+    for (int j = 0; j < NV; j++) {
+      const pz_f4u q = *reinterpret_cast<const pz_f4u*>(x + base + (j * BLOCK + tid) * 4);
 #pragma unroll
       for (int e = 0; e < 4; e++) v[4 * j + e] = q[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; e++) v[4 * j + e] = i + e < A.V ? x[i + e] : -__builtin_inff();
     }
+  } else {
+#pragma unroll
+    for (int j = 0; j < NV; j++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const int i = base + (j * BLOCK + tid) * 4 + e;
+        v[4 * j + e] = i < A.V ? x[i] : -__builtin_inff();
+      }
   }
-  auto id_of = [&](int e) { return base + ((e >> 2) * BLOCK + tid) * 4 + (e & 3); };
+  if (tid < 32) roots[tid] = be_bits(be_roots[tid]);
   if (tid == 0) n_list = 0;
+  pz_lds_barrier();
+  auto id_of = [&](int e) { return base + ((e >> 2) * BLOCK + tid) * 4 + (e & 3); };
+  // (the exponentials as they are, which need no maximum: they are made while the later
+  // loads are on their way)
   float mine = -__builtin_inff();
-  bool bad = false;
-#pragma unroll
-  for (int e = 0; e < N; e++) {
-    mine = fmaxf(mine, v[e]);
-    bad |= !(v[e] < __builtin_inff());
-  }
-  const float wm = pz_wave_max(mine);
-  const bool wb = __ballot(bad) != 0;
-  if (lane == 0) {
-    top[w] = wm;
-    flag[w] = wb;
-  }
-  __syncthreads();
-  float m = top[0];
-  int any = flag[0];
-#pragma unroll
-  for (int i = 1; i < WAVES; i++) {
-    m = fmaxf(m, top[i]);
-    any |= flag[i];
-  }
-  uint64_t* out = A.cand + (size_t)blockIdx.x * A.K;
-  if (any || m == -__builtin_inff()) {
-    for (int i = tid; i < A.K; i += BLOCK) out[i] = 0u;
-    if (tid == 0) A.stat[blockIdx.x] = {0.0, m, any};
-    return;
-  }
   double sum = 0.0;
 #pragma unroll
-  for (int e = 0; e < N; e++) sum += be_exp((double)v[e] - (double)m);
-  sum = be_wave_sum(sum);
-  if (lane == 0) part[w] = sum;
-  // the K best
-  const uint32_t tk = mine == -__builtin_inff() ? 0u : pz_key(mine);
-  const uint32_t T = be_bound<BLOCK>(A.K, hist, [&](auto f) { f(tk); });
-  if (tk >= T)
+  for (int j = 0; j < NV; j++) {
+    // (four at a time: the compiler's mixture of all of them takes three times the registers)
+    asm volatile("" : "+v"(v[4 * j]), "+v"(v[4 * j + 1]), "+v"(v[4 * j + 2]), "+v"(v[4 * j + 3]),
+                 "+v"(sum));
+#pragma unroll
+    for (int e = 4 * j; e < 4 * j + 4; e++) {
+      mine = fmaxf(mine, v[e]);  // (past a NaN, which the other maximum keeps)
+      sum = be_add_exp(sum, (double)__builtin_elementwise_maximum(v[e], BE_LEAST), (be_table)roots);
+    }
+  }
+  float m;
+  const float T = be_bound<BLOCK>(mine, A.K, tops, &m);
+  uint64_t* out = A.cand + (size_t)blockIdx.x * A.K;
+  if (!(fabsf(m) < __builtin_inff())) {  // no finite logit, or an infinite one
+    for (int i = tid; i < A.K; i += BLOCK) out[i] = 0u;
+    if (tid == 0) A.stat[blockIdx.x] = {m > 0.0f ? (double)m : 0.0, m};
+    return;
+  }
+  const float least = fmaxf(T, -3.40282346638528859812e38f);  // (-infinity is never chosen)
+#pragma unroll
+  for (int e = 0; e < N; e++)
+    if (__ballot(v[e] >= least))
+      if (v[e] >= least) {
+        const int i = atomicAdd(&n_list, 1);
+        if (i < BE_CAP) list[i] = be_key(v[e], id_of(e));
+      }
+  const bool plain = fabsf(m) <= BE_PLAIN;
+  if (!plain) {
+    sum = 0.0;
 #pragma unroll
     for (int e = 0; e < N; e++) {
-      const uint32_t k = pz_key(v[e]);
-      if (k >= T && k > BE_NONE) {
-        const int at = atomicAdd(&n_list, 1);
-        if (at < BE_CAP) list[at] = be_key(v[e], id_of(e));
-      }
+      asm volatile("" : "+v"(v[e]), "+v"(sum));
+      sum += be_exp(v[e], m, (be_table)roots);
     }
-  __syncthreads();
+  }
+  sum = be_wave_sum(sum);
+  if (lane == 0) part[w] = sum;
+  pz_lds_barrier();
   const int n = n_list;
   if (tid == 0) {
     double s = part[0];
 #pragma unroll
     for (int i = 1; i < WAVES; i++) s += part[i];
-    A.stat[blockIdx.x] = {s, m, 0};
+    if (plain) s *= exp(-(double)m);
+    A.stat[blockIdx.x] = {s, m};
   }
   for (int i = n + tid; i < A.K; i += BLOCK) out[i] = 0u;
   if (n <= BE_CAP) {
     for (int i = tid; i < n; i += BLOCK) {
       const uint64_t k = list[i];
       int better = 0;
-      for (int j = 0; j < n; j++) better += list[j] > k;
+      for (int j = 0; j < n; j += 8)  // (eight on their way at a time)
+#pragma unroll
+        for (int c = 0; c < 8; c++) better += (list[j + c] > k) & (j + c < n);
       if (better < A.K) out[better] = k;
     }
     return;
@@ -240,9 +296,9 @@ __global__ __launch_bounds__(BLOCK) void k_beam_row(const BeamArgs A) {
       const uint64_t c = __shfl_xor(best, o, 64);
       best = c > best ? c : best;
     }
-    __syncthreads();
+    pz_lds_barrier();
     if (lane == 0) list[w] = best;
-    __syncthreads();
+    pz_lds_barrier();
     best = list[0];
 #pragma unroll
     for (int i = 1; i < WAVES; i++) best = list[i] > best ? list[i] : best;
@@ -258,42 +314,78 @@ struct BeamCand {
   int beam;
 };
 __device__ __forceinline__ bool be_better(const BeamCand& a, const BeamCand& b) {
-  if (a.score != b.score) return a.score > b.score;
-  if (a.beam != b.beam) return a.beam < b.beam;
-  return a.key > b.key;
+  // (no short cuts: they would be branches, and a wait for each member)
+  return (a.score > b.score) |
+         ((a.score == b.score) & ((a.beam < b.beam) | ((a.beam == b.beam) & (a.key > b.key))));
 }
 
 constexpr int BE_JOIN = 1024;  // threads
+constexpr int BE_HELD = 4;     // candidates that a thread keeps
+
+// e / d for e, d < 2^24 and per = 1 / d as a float.
+__device__ __forceinline__ int be_div(int e, int d, float per) {
+  int q = (int)((float)e * per);
+  q -= q * d > e;
+  return q + (e - q * d >= d);
+}
 
 __global__ __launch_bounds__(BE_JOIN) void k_beam_join(const BeamArgs A) {
   constexpr int WAVES = BE_JOIN / 64;
   __shared__ BeamCand list[BE_JCAP];
-  __shared__ uint32_t hist[256];
+  __shared__ double tops[BE_JOIN + 1];
+  __shared__ be_u32x2 roots[32];
   __shared__ double lse[PZ_BEAM_MAX_WIDTH], sum[PZ_BEAM_MAX_WIDTH];
   __shared__ int state[PZ_BEAM_MAX_WIDTH];  // 0: offers nothing, 1: its row, 2: itself
   __shared__ int n_list;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int64_t row0 = (int64_t)blockIdx.x * A.W;
+  const int lists = A.W * A.S, total = lists * A.K;
+  const uint64_t* cand = A.cand + row0 * A.S * A.K;
+  // Candidate e: one of every beam that has ended, then the lists' first ones, their second
+  // ones, ...  A thread keeps BE_HELD of them.  Each wave's are of all lists alike, however
+  // many lists there are, so that be_bound's groups are of equal chances (8 groups of 8
+  // beams, 16 of 16 segments: 100 us with a wave's candidates in a row).
+  auto nth = [&](int i) { return i * BE_JOIN + lane * WAVES + ((w + lane + i) & (WAVES - 1)); };
+  auto load = [&](int e, int* beam) {
+    const int f = e < A.W ? 0 : e - A.W, rank = be_div(f, lists, A.per_list), l = f - rank * lists;
+    *beam = e < A.W ? e : be_div(l, A.S, A.per_segment);
+    return e >= A.W && f < total ? cand[l * A.K + rank] : 0u;
+  };
+  // (on their way beside the beams' sums; what beams that offer nothing left is not used)
+  uint64_t key[BE_HELD];
+  int beam[BE_HELD];
+#pragma unroll
+  for (int i = 0; i < BE_HELD; i++) {
+    key[i] = 0u;
+    beam[i] = 0;
+    if (i * BE_JOIN < total + A.W) key[i] = load(nth(i), &beam[i]);
+  }
+  if (tid < 32) roots[tid] = be_bits(be_roots[tid]);
   if (tid == 0) n_list = 0;
+  pz_lds_barrier();
   for (int b = w; b < A.W; b += WAVES) {
     const int64_t row = row0 + b;
+    const BeamStat* s = A.stat + row * A.S;
+    BeamStat one = {0.0, -__builtin_inff()};
+    if (lane < A.S) one = s[lane];  // (with the next two, whether it counts or not)
     const float sc = A.score[row];
-    int st = !(fabsf(sc) < __builtin_inff()) ? 0 : A.done && A.done[row] ? 2 : 1;
+    const bool ended = A.done && A.done[row];
+    int st = !(fabsf(sc) < __builtin_inff()) ? 0 : ended ? 2 : 1;
     double l = 0.0;
     if (st == 1) {
-      const BeamStat* s = A.stat + row * A.S;
-      float m = -__builtin_inff();
-      bool bad = false;
-      for (int i = lane; i < A.S; i += 64) {
-        bad |= s[i].bad != 0;
+      float m = one.m;
+      bool bad = !(one.sum < __builtin_inf());
+      for (int i = 64 + lane; i < A.S; i += 64) {
+        bad |= !(s[i].sum < __builtin_inf());
         m = fmaxf(m, s[i].m);
       }
       m = pz_wave_max(m);
       if (__ballot(bad) || m == -__builtin_inff()) {
         st = 0;
       } else {
-        for (int i = lane; i < A.S; i += 64)
-          if (s[i].m > -__builtin_inff()) l += s[i].sum * be_exp((double)s[i].m - (double)m);
+        if (one.m > -__builtin_inff()) l = one.sum * be_exp(one.m, m, (be_table)roots);
+        for (int i = 64 + lane; i < A.S; i += 64)
+          if (s[i].m > -__builtin_inff()) l += s[i].sum * be_exp(s[i].m, m, (be_table)roots);
         l = (double)m + log(be_wave_sum(l));
       }
     }
@@ -303,40 +395,52 @@ __global__ __launch_bounds__(BE_JOIN) void k_beam_join(const BeamArgs A) {
       lse[b] = l;
     }
   }
-  __syncthreads();
-  const int per = A.S * A.K, total = A.W * per;
-  const uint64_t* cand = A.cand + row0 * per;
-  // candidate e: of beam e / per, then one of every beam that has ended
-  auto get = [&](int e, BeamCand* c) {
-    if (e < total) {
-      c->beam = e / per;
-      if (state[c->beam] != 1) return false;
-      c->key = cand[e];
-      if (!c->key) return false;
-      c->score = sum[c->beam] + ((double)pz_unkey((uint32_t)(c->key >> 32)) - lse[c->beam]);
-      return true;
-    }
-    c->beam = e - total;
-    c->key = 0xffffffffu - (uint32_t)A.pad;
-    c->score = sum[c->beam];
-    return state[c->beam] == 2;
+  pz_lds_barrier();
+  // the score of what a list of beam b holds (no key: none)
+  auto score_of = [&](int b, uint64_t k) {
+    return state[b] == 1 && k ? sum[b] + ((double)pz_unkey((uint32_t)(k >> 32)) - lse[b])
+                              : -__builtin_inf();
   };
-  // (the nearest float rises with the score; none is infinite after a finite score but
-  // where that is near the largest float, and then -infinity's key is a key like others)
-  const uint32_t T = be_bound<BE_JOIN>(A.K, hist, [&](auto f) {
-    for (int e = tid; e < total + A.W; e += BE_JOIN) {
-      BeamCand c;
-      if (get(e, &c)) f(pz_key((float)c.score));
+  auto take = [&](int e, uint64_t k, int b) -> BeamCand {
+    if (e >= A.W) return {score_of(b, k), k, b};
+    return {state[b] == 2 ? sum[b] : -__builtin_inf(), 0xffffffffu - (uint32_t)A.pad, b};
+  };
+  BeamCand held[BE_HELD];
+  double mine = -__builtin_inf(), top;
+#pragma unroll
+  for (int i = 0; i < BE_HELD; i++) {
+    held[i].score = -__builtin_inf();
+    if (i * BE_JOIN < total + A.W) {
+      held[i] = take(nth(i), key[i], beam[i]);
+      mine = held[i].score > mine ? held[i].score : mine;
     }
-  });
-  for (int e = tid; e < total + A.W; e += BE_JOIN) {
-    BeamCand c;
-    if (get(e, &c) && pz_key((float)c.score) >= T) {
+  }
+  // (a bound that K of those kept reach is one for all)
+  const double T = be_bound<BE_JOIN>(mine, A.K, tops, &top);
+  auto meet = [&](const BeamCand& c) {
+    if (c.score >= T && c.score > -__builtin_inf()) {
       const int at = atomicAdd(&n_list, 1);
       if (at < BE_JCAP) list[at] = c;
     }
-  }
-  __syncthreads();
+  };
+  if (mine >= T)
+#pragma unroll
+    for (int i = 0; i < BE_HELD; i++)
+      if (i * BE_JOIN < total + A.W) meet(held[i]);
+  // the lists' others, each while it reaches the bound (the 32 best of 16 beams of 151936
+  // ids 70 us with all of them looked at, 40 so)
+  if (total + A.W > BE_HELD * BE_JOIN)
+    for (int l = tid; l < lists; l += BE_JOIN) {
+      const int kept = BE_HELD * BE_JOIN - A.W;
+      const int b = be_div(l, A.S, A.per_segment);
+      for (int rank = l < kept ? (kept - l - 1) / lists + 1 : 0; rank < A.K; rank++) {
+        const uint64_t k = cand[l * A.K + rank];
+        const BeamCand c = {score_of(b, k), k, b};
+        if (!(c.score >= T)) break;
+        meet(c);
+      }
+    }
+  pz_lds_barrier();
   const int n = n_list;
   const size_t o = (size_t)blockIdx.x * A.K;
   auto put = [&](int k, const BeamCand& c) {
@@ -357,11 +461,14 @@ __global__ __launch_bounds__(BE_JOIN) void k_beam_join(const BeamArgs A) {
     if (A.done_out) A.done_out[o + k] = 0;
   }
   if (n <= BE_JCAP) {
-    if (tid < n) {
-      const BeamCand c = list[tid];
+    // sixteen threads a candidate
+    for (int i = tid >> 4; i < n; i += BE_JOIN / 16) {
+      const BeamCand c = list[i];
       int better = 0;
-      for (int j = 0; j < n; j++) better += be_better(list[j], c);
-      if (better < A.K) put(better, c);
+      for (int j = tid & 15; j < n; j += 16) better += be_better(list[j], c);
+#pragma unroll
+      for (int s = 1; s < 16; s <<= 1) better += __shfl_xor(better, s, 64);
+      if ((tid & 15) == 0 && better < A.K) put(better, c);
     }
     return;
   }
@@ -369,9 +476,12 @@ __global__ __launch_bounds__(BE_JOIN) void k_beam_join(const BeamArgs A) {
   BeamCand last = {__builtin_inf(), ~0ull, -1};
   for (int k = 0; k < A.K; k++) {
     BeamCand best = {-__builtin_inf(), 0u, 1 << 30};
-    for (int e = tid; e < total + A.W; e += BE_JOIN) {
-      BeamCand c;
-      if (get(e, &c) && be_better(last, c) && be_better(c, best)) best = c;
+    for (int i = 0; i * BE_JOIN < total + A.W; i++) {
+      int b;
+      const uint64_t key = load(nth(i), &b);
+      if (nth(i) >= total + A.W) continue;
+      const BeamCand c = take(nth(i), key, b);
+      if (c.score > -__builtin_inf() && be_better(last, c) && be_better(c, best)) best = c;
     }
 #pragma unroll
     for (int s = 32; s; s >>= 1) {
@@ -576,7 +686,7 @@ extern "C" int pz_beam_select(pz_sampler* s, const float* d_logits, long ld, int
   const int rc = be_workspace(s);
   if (rc != PZ_OK) return rc;
   const int64_t rows = (int64_t)n_groups * W;
-  constexpr int LONG = 512 * 16, SHORT = 256 * 8;
+  constexpr int LONG = 256 * 32, SHORT = 256 * 8;
   const bool few = rows * ((V + LONG - 1) / LONG) < 2 * (int64_t)s->n_cu;
   const int S = few ? (V + SHORT - 1) / SHORT : (V + LONG - 1) / LONG;
   const size_t per = (size_t)W * S * (sizeof(BeamStat) + (size_t)K * sizeof(uint64_t));
@@ -593,6 +703,8 @@ extern "C" int pz_beam_select(pz_sampler* s, const float* d_logits, long ld, int
                         V,
                         S,
                         K,
+                        1.0f / (float)(W * S),
+                        1.0f / (float)S,
                         d_scores + g * W,
                         d_done ? d_done + g * W : nullptr,
                         pad_id,
@@ -604,12 +716,11 @@ extern "C" int pz_beam_select(pz_sampler* s, const float* d_logits, long ld, int
                         d_done_out ? d_done_out + g * K : nullptr,
                         s->d_eos,
                         s->n_eos};
+    const dim3 grid((unsigned)(n * W * S));
     if (few)
-      hipLaunchKernelGGL((k_beam_row<256, 2>), dim3((unsigned)n * W * S), dim3(256), 0, s->stream,
-                         A);
+      hipLaunchKernelGGL((k_beam_row<256, 2>), grid, dim3(256), 0, s->stream, A);
     else
-      hipLaunchKernelGGL((k_beam_row<512, 4>), dim3((unsigned)n * W * S), dim3(512), 0, s->stream,
-                         A);
+      hipLaunchKernelGGL((k_beam_row<256, 8>), grid, dim3(256), 0, s->stream, A);
     PZ_HIP(s, hipGetLastError());
     hipLaunchKernelGGL(k_beam_join, dim3((unsigned)n), dim3(BE_JOIN), 0, s->stream, A);
     PZ_HIP(s, hipGetLastError());

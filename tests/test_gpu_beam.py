@@ -3,7 +3,7 @@ caches (pz_beam_reorder).
 
 Selection, reference in 64 bits: parents, ids and flags are equal; a score is the
 reference's rounded to fp32, whose 64-bit value is off by at most 2^-40 (1 + |score|):
-the exponentials by 2^-45, their sum's logarithm and the sums by a few 2^-53 of the
+the exponentials by 2^-42, their sum's logarithm and the sums by a few 2^-53 of the
 values.  Inputs are random, so that no two candidates of different logits lie that close
 (a draw that did would fail here without a fault; none does).  Reordering is exact."""
 import numpy as np
