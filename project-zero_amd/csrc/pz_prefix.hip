@@ -8,13 +8,18 @@
 // that share it meet each key, in splits of the longest prefix, and each sequence's
 // own.  k_prefix_join adds them up:
 //   M = max m_i,  out = sum_i 2^(c (m_i - M)) o_i / sum_i 2^(c (m_i - M)) l_i.
+// Both parts are one launch: where few rows share a prefix memory bounds both, and where
+// many do the products bound the prefix's part, memory the others.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "../../include/pz_sampler.h"
+#include "pz_prefixplan.h"
 #include "pz_refuse.h"
 #include "pz_sampler_impl.h"
+#include "pz_sharedattn.h"
 #include "pz_treedev.h"
-#include "pz_treeplan.h"
 
 namespace {
 
@@ -102,18 +107,36 @@ void share_out(ARGS& A, int64_t tiles, int S) {
   A.S = (int)((tiles + A.chunk - 1) / A.chunk);
 }
 
-template <int TYPE, int D, int RT, int WAVES>
-void launch_own(pz_sampler* s, OwnArgs& A) {
-  const int64_t groups = ((int64_t)A.B * A.n_kv * A.S + 7) / 8 * 8;
-  hipLaunchKernelGGL((k_tree<TYPE, D, RT, WAVES, OwnArgs>), dim3((unsigned)(groups * A.nblk)),
-                     dim3(64 * WAVES), 0, s->stream, A);
+// The prefixes' part and the sequences' own in one launch: the first `shared` workgroups
+// and the others.
+template <int TYPE, int D, int RTS, int RTO>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D * (1 + (RTS > RTO ? RTS : RTO)) >= 512 ? 1 : 2, 8))) void
+k_prefix(const SharedArgs P, const OwnArgs A, uint32_t shared) {
+  typedef TrLds<D, RTS, 4> S;
+  typedef TrLds<D, RTO, 4> O;
+  __shared__ __align__(16) char buf[sizeof(S) > sizeof(O) ? sizeof(S) : sizeof(O)];
+  if (blockIdx.x < shared)
+    tr_narrow<TYPE, D, RTS, 4>(P, blockIdx.x, threadIdx.x, *reinterpret_cast<S*>(buf));
+  else
+    tr_narrow<TYPE, D, RTO, 4>(A, blockIdx.x - shared, threadIdx.x, *reinterpret_cast<O*>(buf));
 }
-template <int TYPE, int D, int RT>
-void launch_own_wide(pz_sampler* s, OwnArgs& A) {
-  const int64_t groups = ((int64_t)A.B * A.n_kv * A.S + 7) / 8 * 8;
-  hipLaunchKernelGGL((k_tree_wide<TYPE, D, RT, OwnArgs>),
-                     dim3((unsigned)(groups * (A.nblk / TR_WIDE))), dim3(64 * TR_WIDE), 0,
-                     s->stream, A);
+
+// Alike, where many rows share a prefix: there every wave of the other workgroups has a unit
+// of its own, with no barrier.
+template <int TYPE, int D, int RTO>
+__global__ __launch_bounds__(64 * SH_WAVES) __attribute__((amdgpu_waves_per_eu(2, 2))) void
+k_prefix_wide(const SharedArgs P, const OwnArgs A, uint32_t shared) {
+  typedef ShLds<D> S;
+  typedef TrLds<D, RTO, 1> O;
+  __shared__ __align__(16)
+      char buf[sizeof(S) > SH_WAVES * sizeof(O) ? sizeof(S) : SH_WAVES * sizeof(O)];
+  if (blockIdx.x < shared) {
+    sh_attend<TYPE, D>(P, blockIdx.x, *reinterpret_cast<S*>(buf));
+  } else {
+    const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    tr_narrow<TYPE, D, RTO, 1>(A, (blockIdx.x - shared) * SH_WAVES + w, threadIdx.x & 63,
+                               reinterpret_cast<O*>(buf)[w]);
+  }
 }
 
 template <int TYPE, int D>
@@ -124,28 +147,39 @@ int run_part(pz_sampler* s, OwnArgs A, SharedArgs P) {
   const int64_t slots =
       (int64_t)(PZ_TREE_WS / ((size_t)(D + 2) * sizeof(float))) / (int64_t)A.R;
 
-  // each sequence's own keys: as pz_tree_attention would take them
-  const int64_t own = ((int64_t)A.pages.max_blocks << A.pages.shift) / TR_KEYS + 1 +
-                      (A.T + TR_KEYS - 1) / TR_KEYS;
-  const int64_t heads = (int64_t)A.B * A.n_kv;
-  const TrKernel kernel = tr_kernel_for(rows, heads, own, s->n_cu, D, A.ld, A.ld_n);
-  const int own_rows = kernel == TR_WIDE32 ? 256 : kernel == TR_WIDE16 ? 128
-                       : kernel == TR_SOME ? 32 : 16;  // of a workgroup
-  const int own_blocks = (rows + own_rows - 1) / own_rows;
-  share_out(A, own, kernel == TR_FEW_SHORT ? 1
-                    : splits(s, heads * own_blocks, own, slots - 1));
-  A.nblk = kernel == TR_WIDE32 || kernel == TR_WIDE16 ? own_blocks * TR_WIDE : own_blocks;
-
   // the prefixes': the rows of a key head of all who share one
   const int64_t tiles = ((int64_t)P.pages.max_blocks << P.pages.shift) / TR_KEYS + 1;
-  const TrKernel shared =
-      tr_kernel_for((most + P.B - 1) / P.B, (int64_t)P.B * P.n_kv, tiles, s->n_cu, D, P.ld, 0);
-  const int block = shared == TR_WIDE32 ? 256 : shared == TR_WIDE16 ? 128
-                    : shared == TR_SOME ? 32 : 16;
-  const int64_t blocks = most / block + (P.B < A.B ? P.B : A.B);
+  const int64_t heads = (int64_t)A.B * A.n_kv;
+  const int64_t k = P.B < A.B ? P.B : A.B;  // prefixes with a row, at most
+  const PfKernel kernel =
+      pf_kernel_for((most + k - 1) / k, k * P.n_kv, tiles, s->n_cu, D, P.ld, P.pages.shift);
+  const bool wide = kernel == PF_WIDE;
+  const int block = wide ? SH_ROWS * SH_WAVES : kernel == PF_SOME ? 32 : 16;
+  // (k of them: at most (most - k) / block + k row blocks)
+  const int64_t blocks = P.first ? (most - k) / block + k
+                                 : P.B * (((int64_t)P.each * rows + block - 1) / block);
+
+  // each sequence's own keys: 16 or 32 rows of a key head at a time
+  const int64_t own = ((int64_t)A.pages.max_blocks << A.pages.shift) / TR_KEYS + 1 +
+                      (A.T + TR_KEYS - 1) / TR_KEYS;
+  const int own_rows = rows <= 16 ? 16 : 32;
+  A.nblk = (rows + own_rows - 1) / own_rows;
+  const int64_t units = heads * A.nblk;
+  share_out(A, own, splits(s, wide ? (units + SH_WAVES - 1) / SH_WAVES : units, own, slots - 1));
   share_out(P, tiles, splits(s, blocks * P.n_kv, tiles, slots - A.S));
-  if (!pz_launch_fits((blocks * P.n_kv * P.S + 7) / 8 * 8, 512) ||
-      !pz_launch_fits((heads * A.S + 7) / 8 * 8 * A.nblk, 512))
+  if (wide && P.S > 1) {
+    // Both parts at once: the own one reads memory, the other computes, and a CU has one
+    // workgroup of either.  A tile of 64 keys x 256 rows takes a CU 1.9 us, one of 32 own
+    // keys 0.25 us; of the tables' lengths half is there as a rule.
+    const int64_t mine = units * own / 2, theirs = 4 * blocks * P.n_kv * tiles;
+    const int64_t cus = s->n_cu - std::min<int64_t>(s->n_cu / 4, s->n_cu * mine / (mine + theirs));
+    const int64_t S = cus / (blocks * P.n_kv);
+    if (S > 0 && S < P.S) share_out(P, tiles, (int)S);
+  }
+  const int64_t shared = (blocks * P.n_kv * P.S + 7) / 8 * 8;
+  int64_t others = (heads * A.S + 7) / 8 * 8 * A.nblk;
+  if (wide) others = (others + SH_WAVES - 1) / SH_WAVES;
+  if (!pz_launch_fits(shared + others, 512))
     return fail(s, PZ_ERANGE, "B=%d sequences of T=%d nodes", A.B, A.T);
   P.nblk = (int)blocks;
   P.slot = 0;
@@ -153,30 +187,24 @@ int run_part(pz_sampler* s, OwnArgs A, SharedArgs P) {
   P.part = A.part = static_cast<float*>(s->tree_dev);
   P.ml = A.ml = A.part + (size_t)(P.S + A.S) * A.R * D;
 
-  const dim3 grid((unsigned)((blocks * P.n_kv * P.S + 7) / 8 * 8));
-  if (shared == TR_SOME)
-    hipLaunchKernelGGL((k_tree<TYPE, D, 2, 4, SharedArgs>), grid, dim3(256), 0, s->stream, P);
-  else if (shared == TR_FEW || shared == TR_FEW_SHORT)
-    hipLaunchKernelGGL((k_tree<TYPE, D, 1, 4, SharedArgs>), grid, dim3(256), 0, s->stream, P);
-  if (kernel == TR_SOME)
-    launch_own<TYPE, D, 2, 4>(s, A);
-  else if (kernel == TR_FEW || kernel == TR_FEW_SHORT)
-    launch_own<TYPE, D, 1, 4>(s, A);
+  const dim3 grid((unsigned)(shared + others));
+  const uint32_t first = (uint32_t)shared;
+  const hipStream_t st = s->stream;
   if constexpr (D < 256) {
-    if (shared == TR_WIDE32)
-      hipLaunchKernelGGL((k_tree_wide<TYPE, D, 2, SharedArgs>), grid, dim3(64 * TR_WIDE), 0,
-                         s->stream, P);
-    else if (shared == TR_WIDE16)
-      hipLaunchKernelGGL((k_tree_wide<TYPE, D, 1, SharedArgs>), grid, dim3(64 * TR_WIDE), 0,
-                         s->stream, P);
-    if (kernel == TR_WIDE32)
-      launch_own_wide<TYPE, D, 2>(s, A);
-    else if (kernel == TR_WIDE16)
-      launch_own_wide<TYPE, D, 1>(s, A);
+    if (wide && own_rows == 16)
+      hipLaunchKernelGGL((k_prefix_wide<TYPE, D, 1>), grid, dim3(64 * SH_WAVES), 0, st, P, A, first);
+    else if (wide)
+      hipLaunchKernelGGL((k_prefix_wide<TYPE, D, 2>), grid, dim3(64 * SH_WAVES), 0, st, P, A, first);
   }
+  if (kernel == PF_SOME && own_rows == 16)
+    hipLaunchKernelGGL((k_prefix<TYPE, D, 2, 1>), grid, dim3(256), 0, st, P, A, first);
+  else if (kernel == PF_SOME)
+    hipLaunchKernelGGL((k_prefix<TYPE, D, 2, 2>), grid, dim3(256), 0, st, P, A, first);
+  else if (kernel == PF_FEW)  // (a sequence's rows are its prefix's, too: 16 at most)
+    hipLaunchKernelGGL((k_prefix<TYPE, D, 1, 1>), grid, dim3(256), 0, st, P, A, first);
   PZ_HIP(s, hipGetLastError());
-  hipLaunchKernelGGL((k_prefix_join<TYPE, D>), dim3((unsigned)((A.R + 3) / 4)), dim3(256), 0,
-                     s->stream, A, P);
+  hipLaunchKernelGGL((k_prefix_join<TYPE, D>), dim3((unsigned)((A.R + 3) / 4)), dim3(256), 0, st,
+                     A, P);
   PZ_HIP(s, hipGetLastError());
   return PZ_OK;
 }

@@ -241,11 +241,12 @@ struct TrJob {
   int b, h, sp, blk, rows, node0;
 };
 template <int ROWS>
-__device__ __forceinline__ bool tr_job(const TreeArgs& A, int lane, int n_blk, TrJob* J) {
+__device__ __forceinline__ bool tr_job(const TreeArgs& A, uint32_t block, int lane, int n_blk,
+                                       TrJob* J) {
   // the row blocks of one range of keys on one XCD, one after the other
-  const int slot = blockIdx.x >> 3, turn = slot / n_blk;
+  const int slot = block >> 3, turn = slot / n_blk;
   J->blk = slot - turn * n_blk;
-  const int grp = turn * 8 + (blockIdx.x & 7);
+  const int grp = turn * 8 + (block & 7);
   if (grp >= A.B * A.n_kv * A.S) return false;
   // (split by split, so that those that short sequences lack are spread over the
   // XCDs: 32 ragged sequences of up to 4096 positions in 4 splits 89 us, 75 so)
@@ -260,10 +261,11 @@ __device__ __forceinline__ bool tr_job(const TreeArgs& A, int lane, int n_blk, T
 }
 // (a prefix's row blocks follow each other, on one XCD but for its borders)
 template <int ROWS>
-__device__ __forceinline__ bool tr_job(const SharedArgs& A, int lane, int n_blk, TrJob* J) {
+__device__ __forceinline__ bool tr_job(const SharedArgs& A, uint32_t block, int lane, int n_blk,
+                                       TrJob* J) {
   const int total = n_blk * A.n_kv * A.S, per = (total + 7) / 8;
-  const int at = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= per || at >= total) return false;
+  const int at = (block & 7) * per + (block >> 3);
+  if ((int)(block >> 3) >= per || at >= total) return false;
   const int grp = at / n_blk;
   int blk = at - grp * n_blk;
   J->sp = grp / A.n_kv;
@@ -529,23 +531,42 @@ struct TrRows {
   }
 };
 
-template <int TYPE, int D, int RT, int WAVES, class ARGS>
-__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(D * (1 + RT) >= 512 ? 1 : 2, 8))) void
-k_tree(const ARGS A) {
-  constexpr int KS = D / 32, NT = D / 16, NW = NT / 2;  // k steps of S, d tiles, words of V
-  constexpr int ROWS = 16 * RT;
-  constexpr int CH = RT * NT;  // float4s of a lane's results
-  constexpr int QF = RT * KS * 1024;
-  constexpr int LDS_P = ROWS * (TR_KEYS + 1) * 4;
+// LDS of tr_narrow.
+template <int D, int RT, int WAVES>
+struct TrLds {
+  static constexpr int CH = RT * (D / 16);  // float4s of a lane's results
+  static constexpr int QF = RT * (D / 32) * 1024, LDS_P = 16 * RT * (TR_KEYS + 1) * 4;
   // the waves' results meet HALF of them at a time
-  constexpr int HALF = RT > 1 && CH * WAVES > 64 ? 2 : 1, BUF = CH * 1024 / HALF;  // bytes of a wave's
-  constexpr int SH = WAVES * BUF > QF + WAVES * LDS_P ? WAVES * BUF : QF + WAVES * LDS_P;
-  __shared__ __align__(16) char sh[SH];
-  __shared__ float mls[WAVES][ROWS][2];
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  static constexpr int HALF = RT > 1 && CH * WAVES > 64 ? 2 : 1;
+  static constexpr int BUF = CH * 1024 / HALF;  // bytes of a wave's
+  static constexpr int SH = WAVES * BUF > QF + WAVES * LDS_P ? WAVES * BUF : QF + WAVES * LDS_P;
+  __align__(16) char sh[SH];
+  float mls[WAVES][16 * RT][2];
+};
+
+// A workgroup of k_tree (thread tid of it, block its number), or with WAVES = 1 a wave by
+// itself, whatever the others of its workgroup do.
+template <int TYPE, int D, int RT, int WAVES, class ARGS>
+__device__ __forceinline__ void tr_narrow(const ARGS& A, uint32_t block, int tid,
+                                          TrLds<D, RT, WAVES>& lds) {
+  typedef TrLds<D, RT, WAVES> Lds;
+  constexpr int KS = D / 32, NT = D / 16, NW = NT / 2;  // k steps of S, d tiles, words of V
+  constexpr int ROWS = 16 * RT, CH = Lds::CH, QF = Lds::QF, LDS_P = Lds::LDS_P, HALF = Lds::HALF,
+                BUF = Lds::BUF;
+  char* const sh = lds.sh;
+  auto& mls = lds.mls;
+  auto sync = [&]() {
+    if constexpr (WAVES == 1) {
+      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+      __builtin_amdgcn_wave_barrier();
+    } else {
+      __syncthreads();
+    }
+  };
+  const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m = lane & 15, g = lane >> 4;
   TrJob J;
-  if (!tr_job<ROWS>(A, lane, A.nblk, &J)) return;
+  if (!tr_job<ROWS>(A, block, lane, A.nblk, &J)) return;
   const int b = J.b, h = J.h, sp = J.sp, rows = J.rows, row0 = J.blk * ROWS;
   const int node0 = J.node0;
   const int ctx = pz_pages_len(A.pages, A.len[b]),
@@ -654,7 +675,7 @@ k_tree(const ARGS A) {
     }
     *reinterpret_cast<tr_u32x4*>(sh + (f * 64 + lane) * 16) = x;
   }
-  __syncthreads();
+  sync();
 
   TrRows<TYPE, D, RT, false> R;
   R.clear(lane, A.c);
@@ -720,7 +741,7 @@ k_tree(const ARGS A) {
       mls[w][rt * 16 + m][1] = R.l[rt];
     }
   }
-  __syncthreads();  // (and Q is done with)
+  sync();  // (and Q is done with)
   float mt[RT], lt[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; rt++) {
@@ -750,7 +771,7 @@ k_tree(const ARGS A) {
 #pragma unroll
   for (int half = 0; half < HALF; half++) {
     constexpr int RH = RT / HALF, PER = (CH / HALF + WAVES - 1) / WAVES;  // row tiles, float4s of a wave's share
-    if (half) __syncthreads();
+    if (half) sync();
 #pragma unroll
     for (int rt = 0; rt < RH; rt++)
 #pragma unroll
@@ -760,7 +781,7 @@ k_tree(const ARGS A) {
           const tr_f32x4* v = &R.o[half * RH + rt][4 * f];
           *buf(w, (rt * 4 + i) * (NT / 4) + f) = tr_f32x4{v[0][i], v[1][i], v[2][i], v[3][i]};
         }
-    __syncthreads();
+    sync();
 #pragma unroll
     for (int j = 0; j < PER; j++) {
       const int c = w * PER + j, ch = half * (CH / HALF) + c;
@@ -795,6 +816,13 @@ k_tree(const ARGS A) {
   }
 }
 
+template <int TYPE, int D, int RT, int WAVES, class ARGS>
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(D * (1 + RT) >= 512 ? 1 : 2, 8))) void
+k_tree(const ARGS A) {
+  __shared__ TrLds<D, RT, WAVES> lds;
+  tr_narrow<TYPE, D, RT, WAVES>(A, blockIdx.x, threadIdx.x, lds);
+}
+
 // Many rows: the waves of a workgroup own 16 RT rows each and share the keys,
 // whose tiles come straight to LDS through a ring of TR_STAGES -- whole rows of
 // keys and of values, one barrier per tile -- instead of to every wave's
@@ -821,7 +849,7 @@ k_tree_wide(const ARGS A) {
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m = lane & 15, g = lane >> 4;
   TrJob J;
-  if (!tr_job<WAVES * ROWS>(A, lane, ARGS::WHAT == TR_SHARED ? A.nblk : A.nblk / WAVES, &J))
+  if (!tr_job<WAVES * ROWS>(A, blockIdx.x, lane, ARGS::WHAT == TR_SHARED ? A.nblk : A.nblk / WAVES, &J))
     return;
   const int b = J.b, h = J.h, sp = J.sp, rows = J.rows, row0 = (J.blk * WAVES + w) * ROWS;
   const int node0 = J.node0;

@@ -97,6 +97,74 @@ class Shared(Case):
                                         if self.kind == "fp16" else 0.0))
         return out, tol
 
+    def check_tokens(self, out, label=""):
+        """check() for T = 1 without a tree, computed on the GPU, a key head of a prefix's
+        sequences at a time."""
+        t, D, group = self.torch, self.D, self.heads // self.kv
+        _, h, _ = KINDS[self.kind]
+        q = self.q[:, 0, :self.heads * D].cuda().double().reshape(self.B, self.kv, group, D)
+        got = out[:, 0, :self.heads * D].double().reshape(self.B, self.kv, group, D)
+        k, v = self.k.cuda(), self.v.cuda()
+        kn, vn = (x[:, 0].cuda() for x in (self.kn, self.vn))
+
+        def cached(table, n, per):
+            n = min(max(int(n), 0), per * self.page)
+            p = t.arange(n)
+            page = table.long()[p // self.page]
+            ok = (page >= 0) & (page < self.n_pages)
+            return ((t.where(ok, page, 0) * self.page + p % self.page)[ok]).cuda()
+        own = [cached(self.table[b], self.lens[b], self.per) for b in range(self.B)]
+        most = max(len(a) for a in own) + 1
+        at = t.zeros((self.B, most), dtype=t.long, device="cuda")
+        on = t.zeros((self.B, most), dtype=t.bool, device="cuda")
+        for b, a in enumerate(own):
+            at[b, :len(a)], on[b, :len(a) + 1] = a, True
+        for i in sorted(set(self.of)):
+            bs = t.tensor([b for b in range(self.B) if self.of[b] == i]).cuda()
+            pat = cached(self.ptable[i], self.plens[i], self.pper) if i >= 0 else at[0, :0]
+            for hk in range(self.kv):
+                sl = slice(hk * D, hk * D + D)
+                Q = q[bs, hk]                                              # [n, group, D]
+                kp, vp = k[pat, sl].double(), v[pat, sl].double()
+                ko, vo = k[at[bs], sl].double(), v[at[bs], sl].double()    # [n, most, D]
+                last = (on[bs].sum(1) - 1)
+                rows = t.arange(len(bs), device="cuda")
+                ko[rows, last], vo[rows, last] = kn[bs, sl].double(), vn[bs, sl].double()
+                dead = ~on[bs]
+                ko[dead], vo[dead] = 0.0, 0.0
+
+                def over(f, a, b):  # of the prefix's keys, then of its own
+                    x = f(Q).reshape(-1, D) @ f(a).t()
+                    y = f(Q) @ f(b).transpose(1, 2).contiguous()
+                    return t.cat([x.reshape(len(bs), group, -1), y], 2)
+
+                def mix(p, a, b):
+                    n = a.shape[0]
+                    x = p[..., :n].reshape(len(bs) * group, n) @ a
+                    return x.reshape(len(bs), group, D) + p[..., n:].contiguous() @ b
+                s = over(lambda x: x, kp, ko) * self.scale
+                live = t.cat([t.ones((len(bs), len(pat)), dtype=t.bool, device="cuda"), on[bs]], 1)
+                s = t.where(live[:, None], s, -t.inf)
+                p = t.softmax(s, 2)
+                o = mix(p, vp, vo)
+                n = s.shape[2]
+                err = ((D + 2) * 2.0 ** -24 * self.scale * over(t.abs, kp, ko).amax(2)
+                       + 2 * t.where(live[:, None], s.abs(), 0.0).amax(2) * 2.0 ** -24)
+                d = (2 * err + 2.0 ** -20 + n * 2.0 ** -23)[..., None]
+                tol = h * o.abs() + (h + d) * (1 + h) * mix(p, vp.abs(), vo.abs())
+                if self.kind == "fp16":
+                    big = max(float(vp.abs().max()) if len(pat) else 0.0, float(vo.abs().max()))
+                    tol = tol + n * 2.0 ** -33 * big + 2.0 ** -25
+                off = (got[bs, hk] - o).abs() - tol
+                assert (off <= 0).all(), (label, i, hk, off.max())
+
+    def run_tokens(self, s, label=""):
+        d = self.device()
+        self.call(s, d)
+        s.sync()
+        self.check_tokens(d["out"], label)
+        return d["out"]
+
     def device(self):
         d = super().device()
         t = self.torch
@@ -137,10 +205,55 @@ def test_prefixes(torch_cuda, sampler, kind, D, T):
                                           (40, 2, 16, 2), (96, 1, 16, 2), (7, 5, 16, 1)])
 def test_long_prefixes(torch_cuda, sampler, kind, D, B, T, heads, kv):
     """In splits, for few rows and many, chains."""
-    Shared(torch_cuda, kind, [3001], None, [1 + 7 * b % 40 for b in range(B)], T, heads, kv, D, 32,
-           seed=B + T).run(sampler, "one")
-    Shared(torch_cuda, kind, [2049, 777], [1, 1 + B // 2, B], [7 * b % 40 for b in range(B)], T,
-           heads, kv, D, 16, seed=B + T + 7).run(sampler, "two, the first sequence without")
+    for c in (Shared(torch_cuda, kind, [3001], None, [1 + 7 * b % 40 for b in range(B)], T, heads,
+                     kv, D, 32, seed=B + T),
+              # (the first sequence without one)
+              Shared(torch_cuda, kind, [2049, 777], [1, 1 + B // 2, B],
+                     [7 * b % 40 for b in range(B)], T, heads, kv, D, 16, seed=B + T + 7)):
+        (c.run_tokens if T == 1 else c.run)(sampler, c.P)
+
+
+@pytest.mark.parametrize("kind,D", [("bf16", 64), ("bf16", 128), ("fp16", 128), ("fp16", 64)])
+@pytest.mark.parametrize("each", [35, 70, 300])
+def test_many_rows_of_many_heads(torch_cuda, sampler, kind, D, each):
+    """A workgroup for every CU: rows that share keys in LDS, of prefixes that end
+    anywhere in a tile, in one, and before the first; with pages that are missing."""
+    lens = [33, 1, 64, 0] if each == 300 else [200, 129, 1, 64]
+    c = Shared(torch_cuda, kind, lens, None, [b % 3 for b in range(4 * each)], 1, 64, 64, D, 16,
+               seed=each + D)
+    c.run_tokens(sampler, "whole")
+    c.ptable[0, 1] = -1
+    c.ptable[2, 0] = c.n_pages
+    c.run_tokens(sampler, "missing pages")
+
+
+@pytest.mark.parametrize("kind,D", [("bf16", 128), ("fp16", 64)])
+def test_many_rows_of_a_long_prefix(torch_cuda, sampler, kind, D):
+    """In splits, whose borders are anywhere in a tile of 64; tables of more entries than a
+    workgroup keeps at hand, and infinite values where a row's weights are not small."""
+    torch = torch_cuda
+    c = Shared(torch, kind, [8500 + 37], None, [5, 0] * 45, 1, 32, 16, D, 8, seed=D, pspare=0)
+    c.run_tokens(sampler, "splits")
+    c.plens[0] = 8192
+    c.run_tokens(sampler, "whole tiles")
+    c.ptable[0, 700:720] = -1
+    c.ptable[0, 1023] = 2 ** 31 - 1
+    c.run_tokens(sampler, "missing pages")
+    # every score alike, one infinite value
+    c = Shared(torch, kind, [4200], None, [0] * 80, 1, 32, 16, D, 16, seed=D + 1, pspare=120)
+    c.q.zero_()
+    clean = c.run_tokens(sampler, "alike")
+    at = c.pslots(0, torch.tensor([4199]))
+    c.v[at, 3] = float("inf")
+    c.v[at, 2 * D + 1] = float("-inf")
+    d = c.device()
+    c.call(sampler, d)
+    sampler.sync()
+    got, clean = (x.reshape(80, 32, D).float() for x in (d["out"], clean))
+    for h, i, v in ((0, 3, 1.0), (1, 3, 1.0), (4, 1, -1.0), (5, 1, -1.0)):
+        assert (got[:, h, i] == v * float("inf")).all()
+        got[:, h, i] = clean[:, h, i]
+    assert torch.equal(got, clean)
 
 
 @pytest.mark.parametrize("page", [8, 16, 64, 512])
