@@ -288,6 +288,7 @@ __device__ __forceinline__ void sh_attend(const SharedArgs& A, uint32_t block, S
   };
   // the weights of tile t
   auto weights = [&](int t) {
+    float of[RT];  // the sums of this tile's
     if (!full(t)) {
 #pragma unroll
       for (int kt = 0; kt < KT; kt++)
@@ -298,25 +299,42 @@ __device__ __forceinline__ void sh_attend(const SharedArgs& A, uint32_t block, S
           for (int rt = 0; rt < RT; rt++) s[rt][kt][i] = on ? s[rt][kt][i] : -__builtin_inff();
         }
     }
-    // m is raised only where a score passes it by 2^TH (a NaN stays one)
-    float tm[RT];
-    bool up = false;
+    // m is raised only where a lane's weights of a row pass 2^TH (or are NaN), which their
+    // sum tells without the maximum of the scores: then the weights are made again.
+    auto weigh = [&]() {
+      bool pass = false;
 #pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
-      tm[rt] = s[rt][0][0];
+      for (int rt = 0; rt < RT; rt++) {
+        float sum = 0.0f;
 #pragma unroll
-      for (int e = 1; e < 4 * KT; e++)
-        tm[rt] = __builtin_elementwise_maximum(tm[rt], s[rt][e >> 2][e & 3]);
-      up |= (tm[rt] - mx[rt]) * A.c > Y::TH;
-    }
-    if (__ballot(up)) {
+        for (int kt = 0; kt < KT; kt++) {
+          tr_f32x4 p;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const float x = s[rt][kt][i];
+            p[i] = __builtin_amdgcn_exp2f(far ? __builtin_fmaf(x - mx[rt], A.c, Y::OFF)
+                                              : __builtin_fmaf(x, A.c, nb[rt]));
+            sum += p[i];
+          }
+          pf[rt][kt >> 1][2 * (kt & 1)] = Y::pack(p[0], p[1]);
+          pf[rt][kt >> 1][2 * (kt & 1) + 1] = Y::pack(p[2], p[3]);
+        }
+        pass |= !(sum <= Y::MUCH);
+        of[rt] = sum;
+      }
+      return __ballot(pass) != 0;
+    };
+    if (weigh()) {
       bool out = false;
 #pragma unroll
       for (int rt = 0; rt < RT; rt++) {
-        float t = tm[rt];
-        t = fmaxf(t, __shfl_xor(t, 16, 64));
-        t = fmaxf(t, __shfl_xor(t, 32, 64));
-        const float mn = fmaxf(mx[rt], t);
+        float top = s[rt][0][0];
+#pragma unroll
+        for (int e = 1; e < 4 * KT; e++)
+          top = __builtin_elementwise_maximum(top, s[rt][e >> 2][e & 3]);
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float mn = fmaxf(mx[rt], top);
         const float al = tr_lift(mx[rt], mn, A.c);
         mx[rt] = mn;
         l[rt] *= al;
@@ -326,26 +344,11 @@ __device__ __forceinline__ void sh_attend(const SharedArgs& A, uint32_t block, S
       }
       far = __ballot(out) != 0;
 #pragma unroll
-      for (int rt = 0; rt < RT; rt++) nb[rt] = far ? Y::OFF : Y::OFF - mx[rt] * A.c;
+      for (int rt = 0; rt < RT; rt++) nb[rt] = Y::OFF - mx[rt] * A.c;
+      weigh();
     }
-    if (far)
 #pragma unroll
-      for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-        for (int e = 0; e < 4 * KT; e++) s[rt][e >> 2][e & 3] -= mx[rt];
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-      for (int kt = 0; kt < KT; kt++) {
-        tr_f32x4 p;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][kt][i], A.c, nb[rt]));
-          l[rt] += p[i];
-        }
-        pf[rt][kt >> 1][2 * (kt & 1)] = Y::pack(p[0], p[1]);
-        pf[rt][kt >> 1][2 * (kt & 1) + 1] = Y::pack(p[2], p[3]);
-      }
+    for (int rt = 0; rt < RT; rt++) l[rt] += of[rt];
     tie();
   };
   // At the start of interval 2 t + 2: what lies in the place of a position of tile t that

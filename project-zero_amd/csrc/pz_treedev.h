@@ -84,7 +84,7 @@ struct TrType<PZ_BF16> {
   // the weights lie around 2^-40, so that the sums of any 2^31 of them times bf16's
   // largest values stay in fp32 (which has as many exponents: down there the small
   // ones keep their bits to 2^-86 of the largest)
-  static constexpr float OFF = -40.0f, TH = 8.0f;
+  static constexpr float OFF = -40.0f, TH = 8.0f, MUCH = 0x1p-32f;  // 2^(TH + OFF)
   static constexpr uint32_t EXP = 0x7f80u;  // exponent bits of one element
   static constexpr float MOST = 3.38953138925153547590e38f;  // its largest
   __device__ __forceinline__ static tr_f32x4 mfma(tr_u32x4 a, tr_u32x4 b, tr_f32x4 c) {
@@ -103,7 +103,7 @@ template <>
 struct TrType<PZ_F16> {
   // the weights lie around 2^8, so that the small ones of a long sequence keep
   // their bits (fp16 has normal numbers down to 2^-14)
-  static constexpr float OFF = 8.0f, TH = 6.0f;
+  static constexpr float OFF = 8.0f, TH = 6.0f, MUCH = 0x1p14f;
   static constexpr uint32_t EXP = 0x7c00u;
   static constexpr float MOST = 65504.0f;
   __device__ __forceinline__ static tr_f32x4 mfma(tr_u32x4 a, tr_u32x4 b, tr_f32x4 c) {
