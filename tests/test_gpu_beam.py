@@ -394,7 +394,10 @@ def test_pages_outside_the_pool_or_the_cache(torch_cuda, sampler):
 
 
 def test_large_pools(torch_cuda, sampler):
-    """Pools of more words than the workgroup has threads; long tables."""
+    """Pools of more words than the workgroup has threads; long tables; and the last sizes
+    that one launch takes."""
+    for W, per, pool in ((64, 64, 8192), (64, 65, 8192), (2, 3, 8193)):
+        Reordering(torch_cuda, 2, W, per, 8, 1, 64, 2, W + per, pool=pool).run(sampler, pool)
     c = Reordering(torch_cuda, 2, 16, 1200, 8, 1, 64, 1, 5)
     c.run(sampler)
     c = Reordering(torch_cuda, 1, 2, 3, 8, 1, 64, 1, 6, pool=50000)
