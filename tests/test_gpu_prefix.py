@@ -230,7 +230,7 @@ def test_many_rows_of_many_heads(torch_cuda, sampler, kind, D, each):
 @pytest.mark.parametrize("kind,D", [("bf16", 128), ("fp16", 64)])
 def test_many_rows_of_a_long_prefix(torch_cuda, sampler, kind, D):
     """In splits, whose borders are anywhere in a tile of 64; tables of more entries than a
-    workgroup keeps at hand, and infinite values where a row's weights are not small."""
+    workgroup keeps at hand."""
     torch = torch_cuda
     c = Shared(torch, kind, [8500 + 37], None, [5, 0] * 45, 1, 32, 16, D, 8, seed=D, pspare=0)
     c.run_tokens(sampler, "splits")
@@ -239,8 +239,14 @@ def test_many_rows_of_a_long_prefix(torch_cuda, sampler, kind, D):
     c.ptable[0, 700:720] = -1
     c.ptable[0, 1023] = 2 ** 31 - 1
     c.run_tokens(sampler, "missing pages")
-    # every score alike, one infinite value
-    c = Shared(torch, kind, [4200], None, [0] * 80, 1, 32, 16, D, 16, seed=D + 1, pspare=120)
+
+
+@pytest.mark.parametrize("pspare", [120, 250])  # (the table's length tells the kernel)
+@pytest.mark.parametrize("kind,D", [("bf16", 128), ("fp16", 64)])
+def test_one_infinite_value(torch_cuda, sampler, kind, D, pspare):
+    """Every score alike, and two elements of one value infinite: of that column alone."""
+    torch = torch_cuda
+    c = Shared(torch, kind, [4200], None, [0] * 80, 1, 32, 16, D, 16, seed=D + 1, pspare=pspare)
     c.q.zero_()
     clean = c.run_tokens(sampler, "alike")
     at = c.pslots(0, torch.tensor([4199]))
