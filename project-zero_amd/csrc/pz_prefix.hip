@@ -9,7 +9,12 @@
 // own.  k_prefix_join adds them up:
 //   M = max m_i,  out = sum_i 2^(c (m_i - M)) o_i / sum_i 2^(c (m_i - M)) l_i.
 // Both parts are one launch: where few rows share a prefix memory bounds both, and where
-// many do the products bound the prefix's part, memory the others.
+// many do the products bound the prefix's part, memory the others.  32 heads over 8 of 128,
+// bf16, kernel and join in us:
+//   1 prefix of 500 positions, 4 beams of up to 40 of their own: 8.4 + 3.9, the launches and
+//     one tile's way through; 18 as two launches and a join
+//   8 of up to 4096, 8 beams each (119 MB): 28.7 + 5.5, 4.1 TB/s in the first
+//   1 of up to 32768, 256 sequences of up to 512 (104 GFLOP, 374 MB): 176 + 10
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -151,10 +156,11 @@ int run_part(pz_sampler* s, OwnArgs A, SharedArgs P) {
   const int64_t tiles = ((int64_t)P.pages.max_blocks << P.pages.shift) / TR_KEYS + 1;
   const int64_t heads = (int64_t)A.B * A.n_kv;
   const int64_t k = P.B < A.B ? P.B : A.B;  // prefixes with a row, at most
-  const PfKernel kernel =
-      pf_kernel_for((most + k - 1) / k, k * P.n_kv, tiles, s->n_cu, D, P.ld, P.pages.shift);
+  const PfKernel kernel = pf_kernel_for((most + k - 1) / k, k * P.n_kv, tiles, heads, s->n_cu, D,
+                                        P.ld, P.pages.shift);
   const bool wide = kernel == PF_WIDE;
-  const int block = wide ? SH_ROWS * SH_WAVES : kernel == PF_SOME ? 32 : 16;
+  static_assert(SH_ROWS * SH_WAVES == PF_ROWS, "");
+  const int block = wide ? PF_ROWS : kernel == PF_SOME ? 32 : 16;
   // (k of them: at most (most - k) / block + k row blocks)
   const int64_t blocks = P.first ? (most - k) / block + k
                                  : P.B * (((int64_t)P.each * rows + block - 1) / block);
@@ -166,16 +172,16 @@ int run_part(pz_sampler* s, OwnArgs A, SharedArgs P) {
   A.nblk = (rows + own_rows - 1) / own_rows;
   const int64_t units = heads * A.nblk;
   share_out(A, own, splits(s, wide ? (units + SH_WAVES - 1) / SH_WAVES : units, own, slots - 1));
-  share_out(P, tiles, splits(s, blocks * P.n_kv, tiles, slots - A.S));
-  if (wide && P.S > 1) {
-    // Both parts at once: the own one reads memory, the other computes, and a CU has one
-    // workgroup of either.  A tile of 64 keys x 256 rows takes a CU 1.9 us, one of 32 own
-    // keys 0.25 us; of the tables' lengths half is there as a rule.
-    const int64_t mine = units * own / 2, theirs = 4 * blocks * P.n_kv * tiles;
-    const int64_t cus = s->n_cu - std::min<int64_t>(s->n_cu / 4, s->n_cu * mine / (mine + theirs));
-    const int64_t S = cus / (blocks * P.n_kv);
-    if (S > 0 && S < P.S) share_out(P, tiles, (int)S);
+  const int64_t wgs = blocks * P.n_kv;
+  int S;
+  if (wide) {
+    // (32 own keys take a CU 0.25 us; of the table's length half is there as a rule)
+    S = pf_wide_splits(s->n_cu, wgs, tiles, units * own / 8,
+                       std::min<int64_t>({64, slots - A.S, tiles / TR_SHARE}));
+  } else {
+    S = splits(s, wgs, tiles, slots - A.S);
   }
+  share_out(P, tiles, S);
   const int64_t shared = (blocks * P.n_kv * P.S + 7) / 8 * 8;
   int64_t others = (heads * A.S + 7) / 8 * 8 * A.nblk;
   if (wide) others = (others + SH_WAVES - 1) / SH_WAVES;

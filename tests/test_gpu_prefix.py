@@ -246,7 +246,7 @@ def test_many_rows_of_a_long_prefix(torch_cuda, sampler, kind, D):
 def test_one_infinite_value(torch_cuda, sampler, kind, D, pspare):
     """Every score alike, and two elements of one value infinite: of that column alone."""
     torch = torch_cuda
-    c = Shared(torch, kind, [4200], None, [0] * 80, 1, 32, 16, D, 16, seed=D + 1, pspare=pspare)
+    c = Shared(torch, kind, [4200], None, [0] * 40, 1, 32, 16, D, 16, seed=D + 1, pspare=pspare)
     c.q.zero_()
     clean = c.run_tokens(sampler, "alike")
     at = c.pslots(0, torch.tensor([4199]))
@@ -255,7 +255,7 @@ def test_one_infinite_value(torch_cuda, sampler, kind, D, pspare):
     d = c.device()
     c.call(sampler, d)
     sampler.sync()
-    got, clean = (x.reshape(80, 32, D).float() for x in (d["out"], clean))
+    got, clean = (x.reshape(40, 32, D).float() for x in (d["out"], clean))
     for h, i, v in ((0, 3, 1.0), (1, 3, 1.0), (4, 1, -1.0), (5, 1, -1.0)):
         assert (got[:, h, i] == v * float("inf")).all()
         got[:, h, i] = clean[:, h, i]

@@ -12,31 +12,38 @@ FEW, SOME, WIDE = range(3)
 
 
 @pytest.fixture(scope="module")
-def kernel(tmp_path_factory):
+def program(tmp_path_factory):
     exe = tmp_path_factory.mktemp("plan") / "prefix_plan_check"
     subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-I", INC, SRC, "-o", str(exe)],
                    check=True)
 
-    def call(P, B, T, heads, kv, positions, D, ld=4096, shift=4):
-        k = min(P, B)
-        rows = (B * T * (heads // kv) + k - 1) // k
-        args = (rows, k * kv, positions // 32 + 1, D, ld, shift)
+    def run(*args):
         out = subprocess.run([str(exe)] + [str(v) for v in args], capture_output=True, text=True,
                              check=True, timeout=60)
         return int(out.stdout)
+
+    return run
+
+
+@pytest.fixture(scope="module")
+def kernel(program):
+    def call(P, B, T, heads, kv, positions, D, ld=4096, shift=4):
+        k = min(P, B)
+        rows = (B * T * (heads // kv) + k - 1) // k
+        return program(rows, k * kv, positions // 32 + 1, B * kv, D, ld, shift)
 
     return call
 
 
 def test_forms_of_the_gpu_cases(kernel):
     # many rows of many heads: 35, 70 and 300 sequences of each of four prefixes, 64 key heads
-    assert kernel(4, 140, 1, 64, 64, 224, 128) == SOME
-    assert kernel(4, 280, 1, 64, 64, 224, 64) == WIDE
-    assert kernel(4, 1200, 1, 64, 64, 80, 128) == WIDE
+    for each in (35, 70, 300):
+        assert kernel(4, 4 * each, 1, 64, 64, 224, 128) == WIDE
     # many rows of a long prefix
     assert kernel(1, 90, 1, 32, 16, 8544, 128, shift=3) == WIDE
-    assert kernel(1, 80, 1, 32, 16, 6136, 64) == SOME
-    assert kernel(1, 80, 1, 32, 16, 8208, 64) == WIDE
+    # one infinite value
+    assert kernel(1, 40, 1, 32, 16, 6128, 64) == SOME
+    assert kernel(1, 40, 1, 32, 16, 8208, 64) == WIDE
     # long prefixes of few heads
     assert kernel(1, 2, 1, 8, 2, 3008, 128) == FEW
     assert kernel(1, 6, 1, 8, 2, 3008, 128) == SOME
@@ -46,14 +53,33 @@ def test_forms_of_the_gpu_cases(kernel):
 def test_the_ends_of_the_rule(kernel):
     assert kernel(1, 16, 1, 1, 1, 64, 64) == FEW
     assert kernel(1, 17, 1, 1, 1, 64, 64) == SOME
-    assert kernel(256, 256 * 64, 1, 1, 1, 64, 64) == SOME
-    assert kernel(256, 256 * 65, 1, 1, 1, 64, 64) == WIDE
-    assert kernel(256, 256 * 65, 1, 1, 1, 64, 256) == SOME
+    assert kernel(64, 64 * 16, 1, 1, 1, 64, 64) == FEW
+    assert kernel(60, 60 * 17, 1, 1, 1, 64, 64) == SOME   # 1020 of its own
+    assert kernel(61, 61 * 17, 1, 1, 1, 64, 64) == WIDE   # 1037
+    assert kernel(61, 61 * 17, 1, 1, 1, 64, 256) == SOME
     assert kernel(1, 65, 1, 1, 1, 32 * 4094, 64) == SOME
     assert kernel(1, 65, 1, 1, 1, 32 * 4095, 64) == WIDE
+    assert kernel(1, 64, 1, 1, 1, 32 * 4095, 64) == SOME
+    assert kernel(1, 257, 1, 1, 1, 32 * 2046, 64) == SOME  # two blocks of rows
+    assert kernel(1, 257, 1, 1, 1, 32 * 2047, 64) == WIDE
     # more prefixes than sequences: a sequence's rows are the least
     assert kernel(100, 2, 40, 8, 2, 64, 64) == SOME
     # strides and pages whose offsets pass 32 bits
-    assert kernel(256, 256 * 65, 1, 1, 1, 64, 64, ld=1 << 26) == SOME
-    assert kernel(256, 256 * 65, 1, 1, 1, 64, 64, ld=1 << 24, shift=6) == WIDE
-    assert kernel(256, 256 * 65, 1, 1, 1, 64, 64, ld=1 << 24, shift=7) == SOME
+    assert kernel(61, 61 * 17, 1, 1, 1, 64, 64, ld=1 << 26) == SOME
+    assert kernel(61, 61 * 17, 1, 1, 1, 64, 64, ld=1 << 24, shift=6) == WIDE
+    assert kernel(61, 61 * 17, 1, 1, 1, 64, 64, ld=1 << 24, shift=7) == SOME
+
+
+def test_splits(program):
+    """In range, one where there is no room for more, and no CU left over where the work is
+    a whole number of rounds."""
+    for wgs in (1, 8, 32, 100, 256, 5000):
+        for tiles in (1, 8, 129, 1025, 1 << 22):
+            most = min(64, tiles // 8)
+            S = program("splits", wgs, tiles, 0, most)
+            assert 1 <= S <= max(most, 1)
+    assert program("splits", 64, 1025, 0, 0) == 1
+    assert program("splits", 64, 1025, 0, -3) == 1
+    assert program("splits", 256, 1 << 20, 0, 64) in range(1, 65)
+    assert program("splits", 32, 1025, 4608, 64) == 7
+    assert program("splits", 128, 513, 576, 64) == 2
