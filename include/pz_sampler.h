@@ -77,7 +77,8 @@ typedef struct {
 /* Creates a sampler on `device` for batches of up to max_batch rows of up to
  * max_vocab logits and histories of up to max_hist ids (max_hist <= 2048).
  * Allocates all its device memory but the workspaces of verification, of long
- * attention rows and of tree attention, which their first calls allocate.  The largest part is
+ * attention rows, of tree and prefix attention and of beam search, which their first
+ * calls allocate.  The largest part is
  * the scratch that sorts top-p rows with wide nuclei: 16 bytes per id (ids
  * rounded up to a power of two, at most 262144) for each row sorted at once,
  * which is min(max_batch, compute units) rows while that is at most a 64th of
@@ -529,7 +530,8 @@ typedef struct {
  * the prefix's keys together, so that its bytes do not grow with the sequences.
  * Asynchronous on the sampler's stream, in pz_tree_attention's workspace, which the
  * first call of either allocates; after that call it can be captured into a HIP
- * graph.  Calls of both on one sampler, replays included, must be ordered. */
+ * graph.  Calls of both on one sampler, replays included, must be ordered.
+ * n_prefixes is at most 2^20. */
 PZ_API int pz_prefix_attention(pz_sampler *s, const pz_kv_cache *cache,
                                const pz_kv_prefix *prefix, const void *d_kn, const void *d_vn,
                                long ld_n, int B, int T, const int32_t *d_n_nodes,
@@ -570,9 +572,10 @@ typedef struct {
  * and k may be parts of one row (of a fused projection).  d_q_out == d_q with equal
  * strides works in place, and d_k_out == d_k alike; outputs must not overlap the
  * inputs otherwise.  Without queries (n_heads = 0, d_q and d_q_out NULL) or without
- * keys alike.  Pointers and strides that are multiples of 16 bytes, and rot_dim / 2
- * (PZ_ROPE_HALVES) and head_dim likewise, are the quick case.  Asynchronous on the
- * sampler's stream; uses no workspace and can be captured into a HIP graph. */
+ * keys alike.  Angles are meant to stay below 2^50 radians.  Pointers, strides and heads
+ * that are multiples of 16 bytes are the quick case; at most 65536 heads of queries and of
+ * keys, and n times both at most 2^26 - 1.  Asynchronous on the sampler's stream; uses no
+ * workspace and can be captured into a HIP graph. */
 PZ_API int pz_qk_norm_rope(pz_sampler *s, const pz_qk_rope *rope, const void *d_q, long ld_q,
                            const void *d_k, long ld_k, void *d_q_out, long ld_q_out,
                            void *d_k_out, long ld_k_out, int n, const int32_t *d_pos);
@@ -595,7 +598,8 @@ PZ_API int pz_qk_norm_rope(pz_sampler *s, const pz_qk_rope *rope, const void *d_
  * row has no finite logit, a NaN or +infinity, offers nothing: with d_scores of 0,
  * -infinity, -infinity, ... a group starts from one hypothesis.  Where fewer than K
  * are offered the rest reads parent -1, id -1, score -infinity, done 0.  The outputs
- * must not overlap the inputs.  No limit by the sampler's max_batch or max_vocab.
+ * must not overlap the inputs.  No limit by the sampler's max_batch or max_vocab; V is at
+ * most 2^22, n_groups 2^20.
  * Asynchronous on the sampler's stream, in a workspace (PZ_BEAM_WORKSPACE bytes)
  * that the first call allocates; after it, a call can be captured into a HIP graph.
  * Calls of one sampler, replays included, must be ordered. */
@@ -629,7 +633,8 @@ PZ_API int pz_beam_select(pz_sampler *s, const float *d_logits, long ld, int n_g
  * A parent outside [0, W) leaves the beam empty: length 0, a table of -1.  d_blocks_out
  * and d_len_out must not overlap the caches' own tables and lengths: a program keeps
  * two of each and takes them in turn.  Asynchronous on the sampler's stream, in
- * pz_beam_select's workspace (n_groups * W at most PZ_BEAM_MAX_BEAMS); after the first
+ * pz_beam_select's workspace (n_groups * W at most PZ_BEAM_MAX_BEAMS, W * max_blocks
+ * 2^30); after the first
  * call of either it can be captured into a HIP graph.  Calls of both on one sampler,
  * replays included, must be ordered. */
 #define PZ_BEAM_MAX_POOL 262144
