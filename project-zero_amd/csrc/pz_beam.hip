@@ -16,7 +16,7 @@
 //
 // Where more elements tie at the bound than LDS has room for, the K best are taken one by
 // one.  Bound by the read of the logits with the vector instructions (13 an id) close
-// behind: 256 rows of 151936 ids (10% ended, 140 MB) 35 us, 4.0 TB/s, and 6 to join; 47
+// behind: 256 rows of 151936 ids (10% ended, 140 MB) 35-39 us, 4.0-3.6 TB/s, and 6 to join; 47
 // us with a series of 12 terms in place of the table.  Few rows take segments of 2048
 // ids, so that they fill the CUs (8 rows of 128256 ids: 12 us); of 8192 otherwise (64 rows
 // 26 us, 38 in 2048).
