@@ -526,7 +526,8 @@ typedef struct {
  * prefix, then the d_len[b] positions of its own pages and the nodes that it sees, as
  * one softmax.  Arguments, results, rounding and refusals as pz_tree_attention (a
  * softmax weight is rounded against the largest score of the keys that its workgroup
- * reads); also, T * n_heads is at most 32768.  All sequences' rows of a key head meet
+ * reads); also, T * n_heads is at most 32768 (32513
+ * with heads of 256).  All sequences' rows of a key head meet
  * the prefix's keys together, so that its bytes do not grow with the sequences.
  * Asynchronous on the sampler's stream, in pz_tree_attention's workspace, which the
  * first call of either allocates; after that call it can be captured into a HIP

@@ -13,6 +13,7 @@ struct PzRefusal {
 };
 constexpr int PZ_MOST = 1 << 30;  // of ids and list entries, so that 32-bit counters can step past
 constexpr int PZ_MOST_HEADS = 1 << 16;  // so that rows and row lengths fit 32 bits
+constexpr size_t PZ_TREE_WS = (size_t)64 << 20;  // bytes of tree attention's workspace
 constexpr int PZ_MOST_PREFIXES = 1 << 20;
 constexpr int PZ_MOST_ROWS = 1 << 15;  // of a sequence in prefix attention, so that its
                                        // results of two parts fit the workspace
@@ -124,7 +125,10 @@ inline PzRefusal pz_refuse_prefix(const pz_kv_cache* c, const pz_kv_prefix* p, c
   if (!p->d_first && B % p->n_prefixes)
     return {PZ_EINVAL, "without d_first n_prefixes divides B"};
   if (p->n_prefixes > PZ_MOST_PREFIXES) return {PZ_ERANGE, "n_prefixes above 2^20"};
-  if ((int64_t)T * n_heads > PZ_MOST_ROWS) return {PZ_ERANGE, "T * n_heads above 32768"};
+  // (two parts of a sequence's rows are in the workspace)
+  if ((int64_t)T * n_heads > PZ_MOST_ROWS ||
+      2 * (int64_t)T * n_heads * (c->head_dim + 2) * (int64_t)sizeof(float) > (int64_t)PZ_TREE_WS)
+    return {PZ_ERANGE, "T * n_heads above 32768, or 32513 with heads of 256"};
   return PZ_TAKEN;
 }
 

@@ -10,7 +10,6 @@
 #include "pz_params.h"
 
 constexpr int PZ_LMX_ROWS = 256;  // batch rows of one LM-head GEMM launch
-constexpr size_t PZ_TREE_WS = (size_t)64 << 20;  // bytes of tree attention's workspace
 
 struct pz_sampler {
   int device = 0;

@@ -28,7 +28,7 @@ int main() {
     Call a = {{i32, 4, i32, 2, nullptr}, 6, 3, 4, h};
     change(c, a);
     expect(what,
-           pz_refuse_prefix(&c, &a.p, h, h, 128, a.B, a.T, a.heads, 0.125f, a.q, 1L << 23, h,
+           pz_refuse_prefix(&c, &a.p, h, h, 1024, a.B, a.T, a.heads, 0.125f, a.q, 1L << 23, h,
                             1L << 23),
            code);
   };
@@ -47,6 +47,9 @@ int main() {
   prefix("prefix: positions past 32 bits", PZ_ERANGE, P { N; a.p.max_blocks = 1 << 27; });
   prefix("prefix: the most rows", PZ_OK, P { N; a.T = 64; a.heads = 512; });
   prefix("prefix: more rows", PZ_ERANGE, P { N; a.T = 64; a.heads = 514; });
+  // (two parts of a sequence are in the workspace, whatever its heads)
+  prefix("prefix: the most rows of 256", PZ_OK, P { N; c.head_dim = 256; c.ld = 512; a.T = 64; a.heads = 508; });
+  prefix("prefix: more rows of 256", PZ_ERANGE, P { N; c.head_dim = 256; c.ld = 512; a.T = 64; a.heads = 510; });
   prefix("prefix: what the tree refuses", PZ_EINVAL, P { N; c.block_size = 4; });
   prefix("prefix: null q", PZ_EINVAL, P { N; a.q = nullptr; });
   expect("prefix: null prefix",
