@@ -234,6 +234,8 @@ __global__ __launch_bounds__(BLOCK) __attribute__((amdgpu_waves_per_eu(6, 8))) v
       sum = be_add_exp(sum, (double)__builtin_elementwise_maximum(v[e], BE_LEAST), (be_table)roots);
     }
   }
+  // (a NaN is in the sum of a row that has a finite maximum; without one it counts as infinite)
+  if (mine == -__builtin_inff() && sum != sum) mine = __builtin_inff();
   float m;
   const float T = be_bound<BLOCK>(mine, A.K, tops, &m);
   uint64_t* out = A.cand + (size_t)blockIdx.x * A.K;

@@ -161,6 +161,19 @@ def test_masks_and_outliers(torch_cuda, sampler):
         c.run(sampler, 8, label="almost equal")
 
 
+@pytest.mark.parametrize("G,W,V", [(1, 4, 20000), (2, 48, 60000)])
+def test_not_a_number_among_masked_ids(torch_cuda, sampler, G, W, V):
+    """A NaN rules its row out, also where its part of the row has no other logit."""
+    c = Selection(torch_cuda, G, W, V, 5)
+    c.x[:, 1, 100:] = -np.inf
+    c.run(sampler, 4, label="masked")
+    c.x[:, 1, V - 7] = np.nan
+    c.run(sampler, 4, label="and a NaN")
+    c.x[:, 0, 20:] = -np.inf
+    c.x[:, 0, 11000] = np.inf
+    c.run(sampler, 2 * W, label="and an infinity")
+
+
 @pytest.mark.parametrize("V", [5, 2500, 40000])
 def test_ties(torch_cuda, sampler, V):
     """Equal logits, equal beams: lower beams, then lower ids."""
