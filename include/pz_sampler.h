@@ -532,7 +532,7 @@ typedef struct {
  * Asynchronous on the sampler's stream, in pz_tree_attention's workspace, which the
  * first call of either allocates; after that call it can be captured into a HIP
  * graph.  Calls of both on one sampler, replays included, must be ordered.
- * n_prefixes is at most 2^20. */
+ * With d_first n_prefixes is at most 4096. */
 PZ_API int pz_prefix_attention(pz_sampler *s, const pz_kv_cache *cache,
                                const pz_kv_prefix *prefix, const void *d_kn, const void *d_vn,
                                long ld_n, int B, int T, const int32_t *d_n_nodes,

@@ -164,7 +164,7 @@ int run_part(pz_sampler* s, OwnArgs A, SharedArgs P) {
   const int block = wide ? PF_ROWS : kernel == PF_SOME ? 32 : 16;
   // (k of them: at most (most - k) / block + k row blocks)
   const int64_t blocks = P.first ? (most - k) / block + k
-                                 : P.B * (((int64_t)P.each * rows + block - 1) / block);
+                                 : P.B * ((std::min<int64_t>(P.each, P.nb) * rows + block - 1) / block);
 
   // each sequence's own keys: 16 or 32 rows of a key head at a time
   const int64_t own = ((int64_t)A.pages.max_blocks << A.pages.shift) / TR_KEYS + 1 +
@@ -262,13 +262,15 @@ extern "C" int pz_prefix_attention(pz_sampler* s, const pz_kv_cache* cache,
     A.R = (size_t)nb * per;
     SharedArgs P = {};
     static_cast<PartArgs&>(P) = A;
-    P.B = prefix->n_prefixes;
-    P.pages = {cache->n_blocks, shift, prefix->max_blocks};
-    P.blocks = prefix->d_blocks;
-    P.len = prefix->d_len;
     P.first = prefix->d_first;
     P.each = B / prefix->n_prefixes;
-    P.b0 = b0;
+    // (without ranges only the prefixes that these sequences have)
+    const int p0 = P.first ? 0 : b0 / P.each;
+    P.B = P.first ? prefix->n_prefixes : (b0 + nb - 1) / P.each + 1 - p0;
+    P.pages = {cache->n_blocks, shift, prefix->max_blocks};
+    P.blocks = prefix->d_blocks + (size_t)p0 * prefix->max_blocks;
+    P.len = prefix->d_len + p0;
+    P.b0 = b0 - p0 * P.each;
     P.nb = nb;
     A.B = nb;
     A.pages = {cache->n_blocks, shift, cache->max_blocks};

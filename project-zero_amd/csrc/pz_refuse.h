@@ -14,7 +14,7 @@ struct PzRefusal {
 constexpr int PZ_MOST = 1 << 30;  // of ids and list entries, so that 32-bit counters can step past
 constexpr int PZ_MOST_HEADS = 1 << 16;  // so that rows and row lengths fit 32 bits
 constexpr size_t PZ_TREE_WS = (size_t)64 << 20;  // bytes of tree attention's workspace
-constexpr int PZ_MOST_PREFIXES = 1 << 20;
+constexpr int PZ_MOST_PREFIXES = 1 << 12;  // whose ranges are given
 constexpr int PZ_MOST_ROWS = 1 << 15;  // of a sequence in prefix attention, so that its
                                        // results of two parts fit the workspace
 constexpr int PZ_MOST_IDS = 1 << 22;   // of a selection, whose lists of one row are in the workspace
@@ -124,7 +124,9 @@ inline PzRefusal pz_refuse_prefix(const pz_kv_cache* c, const pz_kv_prefix* p, c
     return {PZ_ERANGE, "the prefix's max_blocks * block_size does not fit 32 bits"};
   if (!p->d_first && B % p->n_prefixes)
     return {PZ_EINVAL, "without d_first n_prefixes divides B"};
-  if (p->n_prefixes > PZ_MOST_PREFIXES) return {PZ_ERANGE, "n_prefixes above 2^20"};
+  // (every workgroup looks for its prefix among the ranges, 64 at a time)
+  if (p->d_first && p->n_prefixes > PZ_MOST_PREFIXES)
+    return {PZ_ERANGE, "n_prefixes above 4096 with d_first"};
   // (two parts of a sequence's rows are in the workspace)
   if ((int64_t)T * n_heads > PZ_MOST_ROWS ||
       2 * (int64_t)T * n_heads * (c->head_dim + 2) * (int64_t)sizeof(float) > (int64_t)PZ_TREE_WS)

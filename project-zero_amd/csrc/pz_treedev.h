@@ -270,6 +270,15 @@ __device__ __forceinline__ bool tr_job(const SharedArgs& A, uint32_t block, int 
   int blk = at - grp * n_blk;
   J->sp = grp / A.n_kv;
   J->h = grp - J->sp * A.n_kv;
+  if (!A.first) {  // (as many row blocks each)
+    const int each = ((A.each < A.nb ? A.each : A.nb) * A.T * A.group + ROWS - 1) / ROWS;
+    int lo;
+    J->b = blk / each;
+    J->blk = blk - J->b * each;
+    J->rows = tr_sharers(A, J->b, &lo) * A.T * A.group;
+    J->node0 = lo * A.T;
+    return J->blk * ROWS < J->rows;
+  }
   for (int i0 = 0; i0 < A.B; i0 += 64) {
     int lo = 0, n = 0;
     if (i0 + lane < A.B) n = tr_sharers(A, i0 + lane, &lo);

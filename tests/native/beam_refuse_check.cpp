@@ -43,7 +43,8 @@ int main() {
   prefix("prefix: null lengths", PZ_EINVAL, P { N; a.p.d_len = nullptr; });
   prefix("prefix: empty tables", PZ_EINVAL, P { N; a.p.max_blocks = 0; });
   prefix("prefix: none", PZ_EINVAL, P { N; a.p.n_prefixes = 0; });
-  prefix("prefix: too many", PZ_ERANGE, P { N; a.p.d_first = i32; a.p.n_prefixes = (1 << 20) + 1; });
+  prefix("prefix: too many", PZ_ERANGE, P { N; a.p.d_first = i32; a.p.n_prefixes = 4097; });
+  prefix("prefix: as many without ranges", PZ_OK, P { N; a.B = 5000; a.p.n_prefixes = 5000; });
   prefix("prefix: positions past 32 bits", PZ_ERANGE, P { N; a.p.max_blocks = 1 << 27; });
   prefix("prefix: the most rows", PZ_OK, P { N; a.T = 64; a.heads = 512; });
   prefix("prefix: more rows", PZ_ERANGE, P { N; a.T = 64; a.heads = 514; });

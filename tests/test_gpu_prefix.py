@@ -417,6 +417,35 @@ def test_more_rows_than_the_workspace(torch_cuda, sampler):
         small.check(d["out"][b0:b0 + 3], b0)
 
 
+def test_more_rows_than_the_workspace_in_even_parts(torch_cuda, sampler):
+    """Alike without ranges: turns that begin and end inside a prefix, and hold many; and
+    more prefixes than ranges may name."""
+    T, heads, D = 64, 16, 256
+    for P, B in ((3, 72), (36, 72)):
+        c = Shared(torch_cuda, "bf16", [40, 3, 20] * (P // 3), None, [b % 20 for b in range(B)], T,
+                   heads, 1, D, 16, seed=62)
+        d = c.device()
+        c.call(sampler, d)
+        sampler.sync()
+        each, step = B // P, 2 * 32513 // (2 * T * heads)
+        for b0 in (0, step - 1, step, 2 * step - 1, B - 3):
+            small = Shared(torch_cuda, "bf16", [40] * P, [0] * (P + 1), [0, 0, 0], T, heads, 1, D,
+                           16, seed=62)
+            for n in ("k", "v", "page", "pper", "ptable", "plens", "n_pages", "per"):
+                setattr(small, n, getattr(c, n))
+            small.first = [min(max(i * each - b0, 0), 3) for i in range(P + 1)]
+            small.of = c.of[b0:b0 + 3]
+            small.lens = c.lens[b0:b0 + 3]
+            small.table = c.table[b0:b0 + 3].contiguous()
+            for n in ("q", "kn", "vn"):
+                setattr(small, n, getattr(c, n)[b0:b0 + 3].contiguous())
+            small.check(d["out"][b0:b0 + 3], (P, b0))
+    B = 6000
+    c = Shared(torch_cuda, "bf16", [1 + b % 70 for b in range(B)], None, [b % 3 for b in range(B)],
+               1, 2, 1, 64, 16, seed=63)
+    c.run(sampler, B)
+
+
 def test_as_tree_attention(torch_cuda, sampler):
     """The prefix's pages in each sequence's own table give the same results, within
     both bounds."""
