@@ -526,9 +526,9 @@ typedef struct {
  * prefix, then the d_len[b] positions of its own pages and the nodes that it sees, as
  * one softmax.  Arguments, results, rounding and refusals as pz_tree_attention (a
  * softmax weight is rounded against the largest score of the keys that its workgroup
- * reads); also, T * n_heads is at most 32768 (32513
- * with heads of 256).  All sequences' rows of a key head meet
- * the prefix's keys together, so that its bytes do not grow with the sequences.
+ * reads); also, T * n_heads is at most 32768 (32513 with heads of 256).  All sequences'
+ * rows of a key head meet the prefix's keys together, so that its bytes do not grow with
+ * the sequences.
  * Asynchronous on the sampler's stream, in pz_tree_attention's workspace, which the
  * first call of either allocates; after that call it can be captured into a HIP
  * graph.  Calls of both on one sampler, replays included, must be ordered.
@@ -624,10 +624,11 @@ PZ_API int pz_beam_select(pz_sampler *s, const float *d_logits, long ld, int n_g
  *     layer.  Then pages of its own for positions up to L + ahead - 1 (ahead >= 0: how
  *     many the next step appends; as far as max_blocks goes), then -1.
  *   d_pool [n_groups, n_pool] (n_pool at most PZ_BEAM_MAX_POOL): the pages that the
- *     group's beams may own, ascending, of which a page that no beam's table names any
- *     more is free again: new pages are the lowest free ones, given out in the order
- *     of beams and positions.  W * max_blocks pages always suffice; tables may also
- *     name pages outside the pool (a prompt's), which are shared and never given out.
+ *     group's beams may own, ascending, each once, of which a page that no beam's table
+ *     names any more is free again: new pages are the lowest free ones, given out in the
+ *     order of beams and positions.  W * max_blocks pages always suffice; tables may also
+ *     name pages outside the pool (a prompt's), which are shared and never given out (one
+ *     that L ends in is the first child's to fill, so that no other group may read it).
  *     Groups' pools must not have pages in common.
  *   d_missing [n_groups] or NULL: how many pages the pool lacked (those entries are
  *     -1, and what would have been copied is left out), 0 where all is well.
@@ -635,7 +636,7 @@ PZ_API int pz_beam_select(pz_sampler *s, const float *d_logits, long ld, int n_g
  * and d_len_out must not overlap the caches' own tables and lengths: a program keeps
  * two of each and takes them in turn.  Asynchronous on the sampler's stream, in
  * pz_beam_select's workspace (n_groups * W at most PZ_BEAM_MAX_BEAMS, W * max_blocks
- * 2^30); after the first
+ * at most 2^30); after the first
  * call of either it can be captured into a HIP graph.  Calls of both on one sampler,
  * replays included, must be ordered. */
 #define PZ_BEAM_MAX_POOL 262144

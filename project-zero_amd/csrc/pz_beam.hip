@@ -22,6 +22,8 @@
 // 26 us, 38 in 2048).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "../../include/pz_sampler.h"
 #include "pz_device.h"
 #include "pz_pages.h"
@@ -930,8 +932,10 @@ extern "C" int pz_beam_reorder(pz_sampler* s, const pz_kv_cache* layers, int n_l
   PZ_HIP(s, hipGetLastError());
   for (int l = 0; l < n_layers; l += BE_LAYERS) {
     const unsigned n = (unsigned)(n_layers - l < BE_LAYERS ? n_layers - l : BE_LAYERS);
-    hipLaunchKernelGGL(k_beam_copy, dim3((unsigned)(n_groups * W), 2u * n, (unsigned)parts),
-                       dim3(256), 0, s->stream, layers_of(l));
+    // (most beams copy nothing: workgroups for each part of a page only while they are few)
+    const int64_t z = std::min<int64_t>(parts, BE_MOVES / ((int64_t)n_groups * W * 2 * n) + 1);
+    hipLaunchKernelGGL(k_beam_copy, dim3((unsigned)(n_groups * W), 2u * n, (unsigned)z), dim3(256),
+                       0, s->stream, layers_of(l));
     PZ_HIP(s, hipGetLastError());
   }
   return PZ_OK;

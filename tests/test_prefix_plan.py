@@ -41,6 +41,10 @@ def test_forms_of_the_gpu_cases(kernel):
         assert kernel(4, 4 * each, 1, 64, 64, 224, 128) == WIDE
     # many rows of a long prefix
     assert kernel(1, 90, 1, 32, 16, 8544, 128, shift=3) == WIDE
+    # far pages
+    assert kernel(2, 4, 1, 8, 2, 224, 64) == FEW
+    assert kernel(2, 20, 1, 8, 2, 224, 64) == SOME
+    assert kernel(2, 140, 1, 64, 64, 224, 64) == WIDE
     # one infinite value
     assert kernel(1, 40, 1, 32, 16, 6128, 64) == SOME
     assert kernel(1, 40, 1, 32, 16, 8208, 64) == WIDE
