@@ -259,3 +259,30 @@ def test_search_replayed(torch_cuda):
     for i, (x, y) in enumerate(zip(eager, replayed)):
         for j, (p, q) in enumerate(zip(x, y)):
             assert ro.same_bits(torch, p, q), (i, j)
+
+
+def test_two_searches_at_once(torch_cuda):
+    """Two samplers, their steps under way together: each search as alone."""
+    torch = torch_cuda
+
+    def run(seeds):
+        samplers = [pz.Sampler(B, V) for _ in seeds]
+        for s in samplers:
+            s.set_eos(EOS)
+        searches = [Search(torch, s, seed) for s, seed in zip(samplers, seeds)]
+        torch.cuda.synchronize()
+        for step in range(STEPS):
+            for c in searches:
+                c.step(step & 1)
+                c.carry()
+        torch.cuda.synchronize()
+        said = [[t.cpu().clone() for t in (c.parent, c.nid, c.nscore, c.ndone, c.logits, c.lens[0],
+                                           c.tables[0])] for c in searches]
+        for s in samplers:
+            s.close()
+        return said
+
+    both, alone = run([3, 4]), run([3]) + run([4])
+    for i, (x, y) in enumerate(zip(both, alone)):
+        for j, (p, q) in enumerate(zip(x, y)):
+            assert ro.same_bits(torch, p, q), (i, j)
