@@ -164,13 +164,17 @@ __device__ __forceinline__ F be_bound(F mine, int K, F* lds, F* most) {
   const F v = lds[on ? at : 0];
   F top = -__builtin_inff(), bound = -__builtin_inff();
   int more = 0, least = 0;  // groups above it, groups that it does not pass
-  // (a multiple of four; no short cuts, which would be branches and a wait for each number)
+  // (a multiple of four, aligned; no short cuts, which would be branches and a wait for each)
+  typedef F four __attribute__((ext_vector_type(4)));
 #pragma unroll 4
-  for (int j = 0; j < groups; j++) {
-    const F o = lds[j];
-    more += o > v;
-    least += o >= v;
-    top = o > top ? o : top;
+  for (int j = 0; j < groups; j += 4) {
+    const four o = *reinterpret_cast<const four*>(lds + j);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      more += o[e] > v;
+      least += o[e] >= v;
+      top = o[e] > top ? o[e] : top;
+    }
   }
   const bool is = on & (more < K) & (least >= K);  // (equal ones together)
   const uint64_t kth = __ballot(is);
@@ -191,7 +195,7 @@ __global__ __launch_bounds__(BLOCK) __attribute__((amdgpu_waves_per_eu(6, 8))) v
   __shared__ uint64_t list[BE_CAP + 8];
   __shared__ double part[WAVES];
   __shared__ be_u32x2 roots[32];
-  __shared__ float tops[BLOCK + 1];
+  __shared__ __align__(16) float tops[BLOCK + 1];
   __shared__ int n_list;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int row = blockIdx.x / A.S, seg = blockIdx.x - row * A.S;
@@ -336,7 +340,7 @@ __device__ __forceinline__ int be_div(int e, int d, float per) {
 __global__ __launch_bounds__(BE_JOIN) void k_beam_join(const BeamArgs A) {
   constexpr int WAVES = BE_JOIN / 64;
   __shared__ BeamCand list[BE_JCAP];
-  __shared__ double tops[BE_JOIN + 1];
+  __shared__ __align__(32) double tops[BE_JOIN + 1];
   __shared__ be_u32x2 roots[32];
   __shared__ double lse[PZ_BEAM_MAX_WIDTH], sum[PZ_BEAM_MAX_WIDTH];
   __shared__ int state[PZ_BEAM_MAX_WIDTH];  // 0: offers nothing, 1: its row, 2: itself
