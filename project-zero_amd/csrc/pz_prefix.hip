@@ -14,7 +14,7 @@
 //   1 prefix of 500 positions, 4 beams of up to 40 of their own: 8.4 + 3.9, the launches and
 //     one tile's way through; 18 as two launches and a join
 //   8 of up to 4096, 8 beams each (119 MB): 34 + 5.5, 3.5 TB/s in the first (28.7 from the
-//     caches); twice the splits 5 us more, half of them 7
+//     caches); twice the splits 4 us more, half of them 7
 //   1 of up to 32768, 256 sequences of up to 512 (104 GFLOP, 374 MB): 176 + 10
 #include <hip/hip_runtime.h>
 
@@ -172,7 +172,8 @@ int run_part(pz_sampler* s, OwnArgs A, SharedArgs P) {
   const int own_rows = rows <= 16 ? 16 : 32;
   A.nblk = (rows + own_rows - 1) / own_rows;
   const int64_t units = heads * A.nblk;
-  share_out(A, own, splits(s, wide ? (units + SH_WAVES - 1) / SH_WAVES : units, own, slots - 1));
+  const int64_t own_wgs = wide ? (units + SH_WAVES - 1) / SH_WAVES : units;
+  share_out(A, own, splits(s, own_wgs, own, slots - 1));
   const int64_t wgs = blocks * P.n_kv;
   int S;
   if (wide) {
@@ -183,7 +184,9 @@ int run_part(pz_sampler* s, OwnArgs A, SharedArgs P) {
     S = splits(s, wgs, tiles, slots - A.S);
   }
   share_out(P, tiles, S);
-  const int64_t shared = (blocks * P.n_kv * P.S + 7) / 8 * 8;
+  P.run = (int)((blocks + k - 1) / k);
+  const int64_t runs = (blocks + P.run - 1) / P.run;
+  const int64_t shared = (runs * P.n_kv * P.S + 7) / 8 * 8 * P.run;
   int64_t others = (heads * A.S + 7) / 8 * 8 * A.nblk;
   if (wide) others = (others + SH_WAVES - 1) / SH_WAVES;
   if (!pz_launch_fits(shared + others, 512))

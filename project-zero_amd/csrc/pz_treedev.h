@@ -165,6 +165,7 @@ struct SharedArgs : PartArgs {
   static constexpr TrWhat WHAT = TR_SHARED;
   const int32_t* first;  // [B + 1] sequences, nullptr: `each` of them to a prefix
   int each;
+  int run;     // row blocks of a prefix
   int b0, nb;  // the launch takes nb sequences from b0 on, where q and the results begin
 };
 
@@ -259,17 +260,20 @@ __device__ __forceinline__ bool tr_job(const TreeArgs& A, uint32_t block, int la
   J->node0 = J->b * A.T;
   return J->blk * ROWS < J->rows;
 }
-// (a prefix's row blocks follow each other, on one XCD but for its borders)
+// A prefix's row blocks (`run` of them; with ranges, on average) follow each other on one
+// XCD.  Units of a run and a key head go to the XCDs in turn, split by split, and one further
+// with every turn, so that splits that short prefixes lack leave no XCD idle (16 prefixes of
+// 16384 positions x 16 sequences 196 us in the units' own order, an eighth to each XCD; 186
+// so)
 template <int ROWS>
 __device__ __forceinline__ bool tr_job(const SharedArgs& A, uint32_t block, int lane, int n_blk,
                                        TrJob* J) {
-  const int total = n_blk * A.n_kv * A.S, per = (total + 7) / 8;
-  const int at = (block & 7) * per + (block >> 3);
-  if ((int)(block >> 3) >= per || at >= total) return false;
-  const int grp = at / n_blk;
-  int blk = at - grp * n_blk;
-  J->sp = grp / A.n_kv;
-  J->h = grp - J->sp * A.n_kv;
+  const int slot = block >> 3, turn = slot / A.run, unit = turn * 8 + ((block + turn) & 7);
+  const int v = unit / A.n_kv, runs = (n_blk + A.run - 1) / A.run;
+  J->h = unit - v * A.n_kv;
+  J->sp = v / runs;
+  int blk = (v - J->sp * runs) * A.run + (slot - turn * A.run);
+  if (J->sp >= A.S || blk >= n_blk) return false;
   if (!A.first) {  // (as many row blocks each)
     const int each = ((A.each < A.nb ? A.each : A.nb) * A.T * A.group + ROWS - 1) / ROWS;
     int lo;
