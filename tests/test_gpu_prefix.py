@@ -152,9 +152,15 @@ class Shared(Case):
                        + 2 * t.where(live[:, None], s.abs(), 0.0).amax(2) * 2.0 ** -24)
                 d = (2 * err + 2.0 ** -20 + n * 2.0 ** -23)[..., None]
                 tol = h * o.abs() + (h + d) * (1 + h) * mix(p, vp.abs(), vo.abs())
+                # (bf16: a part's weights are 2^-40 times those against a score m of the row, so
+                # that its largest is at least 2^-40; one below 2^-126, the least normal number,
+                # may be lost, and with it at most 2^-126 / 2^-40 of that part's mean times its
+                # value: for all n keys n 2^-86 max|v|)
+                big = max(float(vp.abs().max()) if len(pat) else 0.0, float(vo.abs().max()))
                 if self.kind == "fp16":
-                    big = max(float(vp.abs().max()) if len(pat) else 0.0, float(vo.abs().max()))
                     tol = tol + n * 2.0 ** -33 * big + 2.0 ** -25
+                else:
+                    tol = tol + n * 2.0 ** -86 * big
                 off = (got[bs, hk] - o).abs() - tol
                 assert (off <= 0).all(), (label, i, hk, off.max())
 
@@ -389,6 +395,43 @@ def test_ends_of_the_range(torch_cuda, sampler):
             # scores far from zero, apart by what the type holds of them
             c = Shared(torch, kind, [200], None, [20] * B, 1, 8, 2, 64, 16, seed=52, sigma=40.0)
             c.run(sampler, (kind, B, "far"))
+
+
+@pytest.mark.parametrize("kind,D", [("bf16", 128), ("fp16", 64)])
+def test_scores_of_many_rows(torch_cuda, sampler, kind, D):
+    """The kernel for many rows: scores far from zero and apart, infinite ones of some rows,
+    rows that are NaN."""
+    torch = torch_cuda
+    c = Shared(torch, kind, [200, 129, 1, 64], None, [b % 3 for b in range(280)], 1, 64, 64, D, 16,
+               seed=81, sigma=80.0 if kind == "bf16" else 60.0)
+    c.run_tokens(sampler, "far")
+    c = Shared(torch, kind, [200, 129, 1, 64], None, [b % 3 for b in range(280)], 1, 64, 64, D, 16,
+               seed=82)
+    at = c.pslots(0, torch.tensor([150]))
+    c.k[at, :D] = 0.0
+
+    def run(first, q=None):
+        c.k[at, 0] = first
+        d = c.device()
+        if q is not None:
+            d["q"][5] = q
+        c.call(sampler, d)
+        sampler.sync()
+        return d["out"][:, 0].reshape(280, 64, D).float()
+    clean, got = run(60000.0), run(float("inf"))
+    up = (c.q[:70, 0, 0] > 0).cuda()
+    assert up.any() and not up.all()
+    assert torch.isnan(got[:70, 0][up]).all() and torch.isfinite(got[:70, 0][~up]).all()
+    # (a score of -infinity is a weight of 0, as one far below the others is)
+    far = (c.q[:70, 0, 0] < -0.5).cuda()
+    assert torch.equal(got[:70, 0][far], clean[:70, 0][far])
+    assert torch.equal(got[:70, 1:], clean[:70, 1:]) and torch.equal(got[70:], clean[70:])
+    # (another row's scores may change which m its neighbours' weights are taken against, and
+    # so their rounding: within the bound)
+    got = run(60000.0, float("nan"))
+    assert torch.isnan(got[5]).all()
+    got[5] = clean[5]
+    c.check_tokens(got.reshape(280, 1, -1), "beside a NaN")
 
 
 def test_more_rows_than_the_workspace(torch_cuda, sampler):
