@@ -13,8 +13,8 @@
 // bf16, kernel and join in us:
 //   1 prefix of 500 positions, 4 beams of up to 40 of their own: 8.4 + 3.9, the launches and
 //     one tile's way through; 18 as two launches and a join
-//   8 of up to 4096, 8 beams each (119 MB): 34 + 5.5, 3.5 TB/s in the first (28.7 from the
-//     caches); twice the splits 4 us more, half of them 7
+//   8 of up to 4096, 8 beams each (119 MB): 33 + 5.5, 3.6 TB/s in the first; twice the
+//     splits 4 us more, half of them 7
 //   1 of up to 32768, 256 sequences of up to 512 (104 GFLOP, 374 MB): 176 + 10
 #include <hip/hip_runtime.h>
 
