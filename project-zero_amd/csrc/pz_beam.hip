@@ -545,6 +545,24 @@ struct ReorderArgs {
 
 constexpr int BE_PLAN = 512;  // threads
 
+// Where `page` is in the pool, -1 if it is not.  Its n pages ascend, each once, so that their
+// distance from the ends is at least what their numbers differ by: a pool of neighbours needs
+// no search (64 beams, tables of 1024 pages: 419 us with one, 104 so; 8 of 2048 97, 37).
+__device__ __forceinline__ int be_find(const int32_t* pool, int n, int32_t page) {
+  if (n == 0) return -1;
+  const int64_t below = (int64_t)page - pool[0], above = (int64_t)pool[n - 1] - page;
+  if (below < 0 || above < 0) return -1;
+  int lo = above < n ? n - 1 - (int)above : 0, hi = below < n ? (int)below : n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (pool[mid] < page)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  return pool[lo] == page ? lo : -1;
+}
+
 __global__ __launch_bounds__(BE_PLAN) void k_beam_plan(const ReorderArgs A) {
   extern __shared__ uint32_t used[];  // a bit a page of the pool
   __shared__ int par[PZ_BEAM_MAX_WIDTH], lens[PZ_BEAM_MAX_WIDTH];
@@ -594,15 +612,8 @@ __global__ __launch_bounds__(BE_PLAN) void k_beam_plan(const ReorderArgs A) {
     const int32_t page = A.blocks[(beam0 + par[b]) * per + col];
     A.blocks_out[beam0 * per + i] = page;
     if (!eldest[b]) continue;  // (its first sibling marks the same)
-    int lo = 0, hi = A.n_pool;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (pool[mid] < page)
-        lo = mid + 1;
-      else
-        hi = mid;
-    }
-    if (lo < A.n_pool && pool[lo] == page) atomicOr(&used[lo >> 5], 1u << (lo & 31));
+    const int at = be_find(pool, A.n_pool, page);
+    if (at >= 0) atomicOr(&used[at >> 5], 1u << (at & 31));
   }
   __syncthreads();
   const int all = from[A.W];
@@ -757,15 +768,8 @@ __global__ __launch_bounds__(BE_MOVE) void k_beam_move(const ReorderArgs R, cons
     const int32_t page = tab[par[b] * per + col];
     if (tables) R.blocks_out[beam0 * per + i] = page;
     if (!eldest[b]) continue;  // (its first sibling marks the same)
-    int lo = 0, hi = R.n_pool;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (pool[mid] < page)
-        lo = mid + 1;
-      else
-        hi = mid;
-    }
-    if (lo < R.n_pool && pool[lo] == page) atomicOr(&used[lo >> 5], 1u << (lo & 31));
+    const int at = be_find(pool, R.n_pool, page);
+    if (at >= 0) atomicOr(&used[at >> 5], 1u << (at & 31));
   }
   __syncthreads();
   // the free pages' numbers: a word a thread
