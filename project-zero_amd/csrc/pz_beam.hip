@@ -684,10 +684,9 @@ __global__ __launch_bounds__(256) void k_beam_copy(const CopyArgs A) {
   int64_t src, dst;
   if (!pz_pages_slot(A.pages, c.x, 0, &src) || !pz_pages_slot(A.pages, c.y, 0, &dst)) return;
   uint16_t* buf = A.buf[blockIdx.y >> 1][blockIdx.y & 1];
-  const int per = A.row / 8, n = c.z * per;  // 16-byte pieces
-  for (int i = blockIdx.z * 256 + threadIdx.x; i < n; i += gridDim.z * 256) {
-    const int p = i / per;
-    const size_t at = (size_t)p * A.ld + (size_t)(i - p * per) * 8;
+  // (16-byte pieces)
+  for (PzPieces i(A.row / 8, blockIdx.z * 256 + threadIdx.x, gridDim.z * 256); i.p < c.z; i.next()) {
+    const size_t at = (size_t)i.p * A.ld + (size_t)i.j * 8;
     *reinterpret_cast<be_u32x4*>(buf + dst * A.ld + at) =
         *reinterpret_cast<const be_u32x4*>(buf + src * A.ld + at);
   }
@@ -828,10 +827,9 @@ __global__ __launch_bounds__(BE_MOVE) void k_beam_move(const ReorderArgs R, cons
     return;
   const int rest = job - mine * (buffers * parts), which = rest / parts, part = rest - which * parts;
   uint16_t* buf = C.buf[which >> 1][which & 1];
-  const int row = C.row / 8, all = rem * row;  // 16-byte pieces
-  for (int i = part * BE_MOVE + tid; i < all; i += parts * BE_MOVE) {
-    const int p = i / row;
-    const size_t o = (size_t)p * C.ld + (size_t)(i - p * row) * 8;
+  // (16-byte pieces)
+  for (PzPieces i(C.row / 8, part * BE_MOVE + tid, parts * BE_MOVE); i.p < rem; i.next()) {
+    const size_t o = (size_t)i.p * C.ld + (size_t)i.j * 8;
     *reinterpret_cast<be_u32x4*>(buf + dst * C.ld + o) =
         *reinterpret_cast<const be_u32x4*>(buf + src * C.ld + o);
   }
