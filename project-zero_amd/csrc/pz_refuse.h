@@ -175,6 +175,13 @@ inline PzRefusal pz_refuse_rope(const pz_qk_rope* r, const void* d_q, long ld_q,
   return PZ_TAKEN;
 }
 
+// Whether the rotation's kernel with four waves a workgroup takes n tokens of `heads` heads: a
+// wave for each is the most that it launches, whose workgroups are rounded up.  (So the three
+// largest calls that are taken go to the kernel with one.)
+inline bool pz_rope_in_fours(int n, int heads) {
+  return pz_launch_fits(((int64_t)n * heads + 3) / 4, 256);
+}
+
 inline PzRefusal pz_refuse_select(const float* d_logits, long ld, int n_groups, int W, int V,
                                   const float* d_scores, int K, const int32_t* d_parent,
                                   const int32_t* d_ids, const float* d_scores_out) {

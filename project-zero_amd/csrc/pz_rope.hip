@@ -306,7 +306,7 @@ int lanes(pz_sampler* s, RopeArgs& A) {
 template <int TYPE>
 int run(pz_sampler* s, RopeArgs& A, int layout) {
   constexpr int E = RopeType<TYPE>::E;
-  bool quick = A.D % E == 0 && A.D / E <= 128;
+  bool quick = A.D % E == 0 && A.D / E <= 128 && pz_rope_in_fours(A.n, A.heads[0] + A.heads[1]);
   for (int i = 0; i < 2; i++)
     quick = quick && (!A.heads[i] || (pz_aligned16(A.in[i]) && pz_aligned16(A.out[i]) &&
                                       A.ld_in[i] % E == 0 && A.ld_out[i] % E == 0));
