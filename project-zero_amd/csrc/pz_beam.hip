@@ -3,9 +3,10 @@
 //
 // Selection.  score[w, i] = d_scores[w] + (x[w, i] - lse_w), lse_w = log sum_j exp(x[w, j]).
 // Beams of a group lie close together, so that lse decides between their candidates: it is
-// held in 64 bits, its exponentials to 2^-43.  (A 64-bit fma takes a wave as long as a
-// 32-bit one here.)  Within a beam the score rises with the logit, so that a row's K best
-// are the K largest logits:
+// held in 64 bits.  Exponentials are off by at most 2^-43 (pz_beamexp.h), the factors that
+// join a row's segments alike, lse by 2^-42 and a few 2^-53 of its value.  (A 64-bit fma takes
+// a wave as long as a 32-bit one here.)  Within a beam the score rises with the logit, so that
+// a row's K best are the K largest logits:
 //
 //   * k_beam_row: a workgroup a segment of a row, which it reads once, to registers:
 //     maximum, sum of exponentials, and its K best as keys (order key of the logit, then
@@ -25,6 +26,7 @@
 #include <algorithm>
 
 #include "../../include/pz_sampler.h"
+#include "pz_beamexp.h"
 #include "pz_device.h"
 #include "pz_pages.h"
 #include "pz_refuse.h"
@@ -58,47 +60,11 @@ struct BeamArgs {
   int n_eos;
 };
 
-// exp(x) = 2^(n / 32) exp(r), n the whole number nearest to 32 x / ln 2 (which the sum with
-// 1.5 2^52 leaves in its last bits) and |r| <= ln 2 / 64: 2^(n % 32 / 32) from a table, n / 32
-// into its exponent, and exp(r) from its series up to r^4, with r^5 / 120 replaced by
-// the cubic that is nearest on the interval (Chebyshev's): 2^-43 is left.
-// (The table: the bits of 2^(i / 32) less i 2^47, so that all of n may be added.)
-__constant__ const uint64_t be_roots[32] = {
-    0x3ff0000000000000ull, 0x3fefd9b0d3158574ull, 0x3fefb5586cf9890full, 0x3fef9301d0125b51ull,
-    0x3fef72b83c7d517bull, 0x3fef54873168b9aaull, 0x3fef387a6e756238ull, 0x3fef1e9df51fdee1ull,
-    0x3fef06fe0a31b715ull, 0x3feef1a7373aa9cbull, 0x3feedea64c123422ull, 0x3feece086061892dull,
-    0x3feebfdad5362a27ull, 0x3feeb42b569d4f82ull, 0x3feeab07dd485429ull, 0x3feea47eb03a5585ull,
-    0x3feea09e667f3bcdull, 0x3fee9f75e8ec5f74ull, 0x3feea11473eb0187ull, 0x3feea589994cce13ull,
-    0x3feeace5422aa0dbull, 0x3feeb737b0cdc5e5ull, 0x3feec49182a3f090ull, 0x3feed503b23e255dull,
-    0x3feee89f995ad3adull, 0x3feeff76f2fb5e47ull, 0x3fef199bdd85529cull, 0x3fef3720dcef9069ull,
-    0x3fef5818dcfba487ull, 0x3fef7c97337b9b5full, 0x3fefa4afa2a490daull, 0x3fefd0765b6e4540ull};
-constexpr double BE_PER = 46.1662413084468290355, BE_STEP = 0.0216608493924982909193;
-constexpr double BE_C1 = 0.999999999964169676946, BE_C3 = 0.166667888521865636702;
+// (The logits' exponentials: pz_beamexp.h.)
 constexpr float BE_PLAIN = 500.0f;  // largest |m| whose exponentials are taken as they are
 constexpr float BE_LEAST = -650.0f;  // smaller logits count as this beside such an m (10^-65 of it)
-typedef uint32_t be_u32x2 __attribute__((ext_vector_type(2)));  // low, high
 typedef __attribute__((address_space(3))) const be_u32x2* be_table;
 __device__ __forceinline__ be_u32x2 be_bits(uint64_t v) { return __builtin_bit_cast(be_u32x2, v); }
-// sum + exp(d), |d| <= 700
-__device__ __forceinline__ double be_add_exp(double sum, double d, be_table roots) {
-  constexpr double ROUND = 6755399441055744.0;  // 1.5 2^52
-  const double t = __builtin_fma(d, BE_PER, ROUND), n = t - ROUND;
-  const double r = __builtin_fma(n, -BE_STEP, d);
-  const uint32_t k = (uint32_t)__builtin_bit_cast(uint64_t, t);
-  be_u32x2 root = roots[k & 31u];
-  root[1] += k << 15;
-  const double scale = __builtin_bit_cast(double, root);
-  double p = __builtin_fma(r, 1.0 / 24.0, BE_C3);
-  p = __builtin_fma(r, p, 0.5);
-  p = __builtin_fma(r, p, BE_C1);
-  p = __builtin_fma(r, p, 1.0);
-  return __builtin_fma(p, scale, sum);
-}
-// exp(x - m), x <= m
-__device__ __forceinline__ double be_exp(float x, float m, be_table roots) {
-  const double d = (double)x - (double)m;
-  return be_add_exp(0.0, d < -700.0 ? -700.0 : d, roots);  // (10^-304 at least; a NaN stays)
-}
 
 __device__ __forceinline__ double be_wave_sum(double v) {
 #pragma unroll
