@@ -2,7 +2,7 @@
 //
 // As k_tree_wide (pz_treedev.h): S^T = K Q^T and O^T = V^T P^T on 16x16x32 matrix
 // instructions, keys and values through LDS, running maximum and sum of a row in the lanes
-// that hold it.  What is different, since nothing but full tiles of one prefix comes by:
+// that hold it.  What is different, since nothing but one prefix's positions comes by:
 //
 //   * a tile is 64 keys, and a step of it has two phases: the products (the last tile's
 //     weights with its values, this one's keys with the queries) and the weights.  The
@@ -83,7 +83,8 @@ __device__ __forceinline__ void sh_attend(const SharedArgs& A, uint32_t block, S
   const int h = J.h, sp = J.sp, rows = J.rows, row0 = (J.blk * SH_WAVES + w) * SH_ROWS;
   const bool idle = row0 >= rows;  // (a wave past the last row loads only)
   const int ctx = pz_pages_len(A.pages, A.len[J.b]);
-  // (splits are counted in tiles of TR_KEYS, an even number of them)
+  // (splits are counted in tiles of TR_KEYS; where a share is an odd number of them, the last
+  // tile here of every split is half full, as that of a prefix may be)
   const int chunk = tr_chunk(A, J.b, lane), ntl = tr_tiles(A, J.b);
   const int tl0 = sp * chunk, tl1 = ntl - tl0 < chunk ? ntl : tl0 + chunk;
   if (tl0 >= ntl) return;
