@@ -15,15 +15,20 @@
 //     LDS, where each counts those that are better.
 //   * k_beam_join: a workgroup a group; the same over its beams' candidates.
 //
-// Where more elements tie at the bound than LDS has room for, the K best are taken one by
-// one.  Bound by the read of the logits with the vector instructions (13 an id) close
-// behind: 256 rows of 151936 ids (10% ended, 140 MB) 35-39 us, 4.0-3.6 TB/s, and 6 to join; 47
-// us with a series of 12 terms in place of the table.  Few rows take segments of 2048
-// ids, so that they fill the CUs (8 rows of 128256 ids: 12 us); of 8192 otherwise (64 rows
-// 26 us, 38 in 2048).
+// Where many more than K reach the bound (masks of low logits that are finite, of which all tie;
+// beams whose scores lie far apart) the join takes a better one from those that have met, and
+// either kernel takes the K best one by one where that is less work (be_counted).  1 x 4 beams
+// of 128256 ids, 8 best: 11 us, 16 where a thousandth of the ids is above the mask; 16 beams, 128
+// best: 46, and 85 where their scores are 6 apart (365 and 9700 before).
+//
+// Bound by the read of the logits with the vector instructions (13 an id) close behind: 256
+// rows of 151936 ids (10% ended, 140 MB) 35-39 us, 4.0-3.6 TB/s, and 6 to join; 47 us with a
+// series of 12 terms in place of the table.  Few rows take segments of 2048 ids, so that they
+// fill the CUs (8 rows of 128256 ids: 12 us); of 8192 otherwise (64 rows 26 us, 38 in 2048).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "../../include/pz_sampler.h"
 #include "pz_beamexp.h"
@@ -36,6 +41,8 @@ namespace {
 
 constexpr int BE_CAP = 2048;   // elements of a segment that meet in LDS
 constexpr int BE_JCAP = 1024;  // candidates of a group that do
+constexpr int BE_LONG = 256 * 32, BE_SHORT = 256 * 8;  // ids of a segment
+constexpr int BE_LISTS = PZ_BEAM_MAX_WIDTH * (PZ_MOST_IDS / BE_LONG + 1);  // of a group, and one a beam
 
 struct BeamStat {
   double sum;  // of exp(x - m); not finite where a logit is NaN or +infinity
@@ -47,6 +54,7 @@ struct BeamArgs {
   long ld;
   int W, V, S, K;  // beams, ids, segments of a row
   float per_list, per_segment;  // 1 / (W S), 1 / S
+  int row_most, join_most;      // that are counted against each other (be_counted)
   const float* score;
   const uint8_t* done;
   int32_t pad;
@@ -245,7 +253,7 @@ __global__ __launch_bounds__(BLOCK) __attribute__((amdgpu_waves_per_eu(6, 8))) v
     A.stat[blockIdx.x] = {s, m};
   }
   for (int i = n + tid; i < A.K; i += BLOCK) out[i] = 0u;
-  if (n <= BE_CAP) {
+  if (n <= A.row_most) {
     for (int i = tid; i < n; i += BLOCK) {
       const uint64_t k = list[i];
       int better = 0;
@@ -295,6 +303,9 @@ __device__ __forceinline__ bool be_better(const BeamCand& a, const BeamCand& b) 
 
 constexpr int BE_JOIN = 1024;  // threads
 constexpr int BE_HELD = 4;     // candidates that a thread keeps
+constexpr int BE_JLDS = std::max<int>(BE_JCAP * sizeof(BeamCand) + (BE_JOIN + 1) * sizeof(double),
+                                      BE_JOIN / 64 * sizeof(BeamCand) + BE_LISTS);
+static_assert(BE_JCAP * sizeof(BeamCand) % 32 == 0, "four of tops together");
 
 // e / d for e, d < 2^24 and per = 1 / d as a float.
 __device__ __forceinline__ int be_div(int e, int d, float per) {
@@ -305,8 +316,11 @@ __device__ __forceinline__ int be_div(int e, int d, float per) {
 
 __global__ __launch_bounds__(BE_JOIN) void k_beam_join(const BeamArgs A) {
   constexpr int WAVES = BE_JOIN / 64;
-  __shared__ BeamCand list[BE_JCAP];
-  __shared__ __align__(32) double tops[BE_JOIN + 1];
+  // list and tops; or, where candidates are taken one by one, how many of each list are
+  __shared__ __align__(32) char mem[BE_JLDS];
+  BeamCand* const list = reinterpret_cast<BeamCand*>(mem);
+  double* const tops = reinterpret_cast<double*>(mem + BE_JCAP * sizeof(BeamCand));
+  uint8_t* const taken = reinterpret_cast<uint8_t*>(mem + WAVES * sizeof(BeamCand));
   __shared__ be_u32x2 roots[32];
   __shared__ double lse[PZ_BEAM_MAX_WIDTH], sum[PZ_BEAM_MAX_WIDTH];
   __shared__ int state[PZ_BEAM_MAX_WIDTH];  // 0: offers nothing, 1: its row, 2: itself
@@ -390,32 +404,50 @@ __global__ __launch_bounds__(BE_JOIN) void k_beam_join(const BeamArgs A) {
     }
   }
   // (a bound that K of those kept reach is one for all)
-  const double T = be_bound<BE_JOIN>(mine, A.K, tops, &top);
+  double T = be_bound<BE_JOIN>(mine, A.K, tops, &top);
   auto meet = [&](const BeamCand& c) {
     if (c.score >= T && c.score > -__builtin_inf()) {
       const int at = atomicAdd(&n_list, 1);
       if (at < BE_JCAP) list[at] = c;
     }
   };
+  // those of list l from `rank` on, while they reach the bound (the 32 best of 16 beams of
+  // 151936 ids 70 us with all of them looked at, 40 so)
+  auto open = [&](int l, int rank) {
+    const int b = be_div(l, A.S, A.per_segment);
+    for (; rank < A.K; rank++) {
+      const uint64_t k = cand[l * A.K + rank];
+      const BeamCand c = {score_of(b, k), k, b};
+      if (!(c.score >= T)) break;
+      meet(c);
+    }
+  };
   if (mine >= T)
 #pragma unroll
     for (int i = 0; i < BE_HELD; i++)
       if (i * BE_JOIN < total + A.W) meet(held[i]);
-  // the lists' others, each while it reaches the bound (the 32 best of 16 beams of 151936
-  // ids 70 us with all of them looked at, 40 so)
-  if (total + A.W > BE_HELD * BE_JOIN)
+  if (total + A.W > BE_HELD * BE_JOIN)  // the lists' others
     for (int l = tid; l < lists; l += BE_JOIN) {
       const int kept = BE_HELD * BE_JOIN - A.W;
-      const int b = be_div(l, A.S, A.per_segment);
-      for (int rank = l < kept ? (kept - l - 1) / lists + 1 : 0; rank < A.K; rank++) {
-        const uint64_t k = cand[l * A.K + rank];
-        const BeamCand c = {score_of(b, k), k, b};
-        if (!(c.score >= T)) break;
-        meet(c);
-      }
+      open(l, l < kept ? (kept - l - 1) / lists + 1 : 0);
     }
   pz_lds_barrier();
-  const int n = n_list;
+  int n = n_list;
+  // More than there is room for (where some beams' scores are far above the others', the bound
+  // is that of all lists' first ones): the K-th of those that have met is a better one, but
+  // where they tie.
+  static_assert(BE_JCAP == BE_JOIN, "one of them a thread");
+  while (n > BE_JCAP) {
+    const double better = be_bound<BE_JOIN>(list[tid].score, A.K, tops, &top);
+    if (!(better > T)) break;
+    T = better;
+    if (tid == 0) n_list = 0;
+    pz_lds_barrier();
+    if (tid < A.W) meet(take(tid, 0u, tid));
+    for (int l = tid; l < lists; l += BE_JOIN) open(l, 0);
+    pz_lds_barrier();
+    n = n_list;
+  }
   const size_t o = (size_t)blockIdx.x * A.K;
   auto put = [&](int k, const BeamCand& c) {
     const int32_t id = (int32_t)(0xffffffffu - (uint32_t)c.key);
@@ -434,7 +466,7 @@ __global__ __launch_bounds__(BE_JOIN) void k_beam_join(const BeamArgs A) {
     A.score_out[o + k] = -__builtin_inff();
     if (A.done_out) A.done_out[o + k] = 0;
   }
-  if (n <= BE_JCAP) {
+  if (n <= A.join_most) {
     // sixteen threads a candidate
     for (int i = tid >> 4; i < n; i += BE_JOIN / 16) {
       const BeamCand c = list[i];
@@ -446,17 +478,27 @@ __global__ __launch_bounds__(BE_JOIN) void k_beam_join(const BeamArgs A) {
     }
     return;
   }
-  // one by one
-  BeamCand last = {__builtin_inf(), ~0ull, -1};
-  for (int k = 0; k < A.K; k++) {
-    BeamCand best = {-__builtin_inf(), 0u, 1 << 30};
-    for (int i = 0; i * BE_JOIN < total + A.W; i++) {
-      int b;
-      const uint64_t key = load(nth(i), &b);
-      if (nth(i) >= total + A.W) continue;
-      const BeamCand c = take(nth(i), key, b);
-      if (c.score > -__builtin_inf() && be_better(last, c) && be_better(c, best)) best = c;
+  // one by one: the best of the threads' best.  A thread has every BE_JOIN-th list (and those of
+  // one candidate, the ended beams'), each of which is in order; who gave the best takes its
+  // list's next.
+  const int all = lists + A.W;
+  pz_lds_barrier();
+  for (int l = tid; l < all; l += BE_JOIN) taken[l] = 0;  // (a thread's own)
+  BeamCand own;
+  int from = 0;  // whose the best is
+  auto look = [&]() {
+    own = {-__builtin_inf(), 0u, 1 << 30};
+    for (int l = tid; l < all; l += BE_JOIN) {
+      const int rank = taken[l];
+      if (rank == (l < lists ? A.K : 1)) continue;
+      const BeamCand c = l < lists ? take(A.W, cand[l * A.K + rank], be_div(l, A.S, A.per_segment))
+                                   : take(l - lists, 0u, l - lists);
+      if (c.score > -__builtin_inf() && be_better(c, own)) own = c, from = l;
     }
+  };
+  look();
+  for (int k = 0; k < A.K; k++) {
+    BeamCand best = own;
 #pragma unroll
     for (int s = 32; s; s >>= 1) {
       const BeamCand c = {__shfl_xor(best.score, s, 64), __shfl_xor(best.key, s, 64),
@@ -470,8 +512,24 @@ __global__ __launch_bounds__(BE_JOIN) void k_beam_join(const BeamArgs A) {
     for (int i = 1; i < WAVES; i++)
       if (be_better(list[i], best)) best = list[i];
     if (tid == 0) put(k, best);
-    last = best;
+    if (best.beam == own.beam && best.key == own.key) {
+      taken[from]++;
+      look();
+    }
   }
+}
+
+// Up to how many are counted against each other, each by those that are better, rather than
+// taken one by one: n of a segment take ceil(n / 256) n 22 ns, one by one 0.5 us each of the K
+// (2048 that tie, 8 best: 355 us and 4); of a group n^2 0.1 ns and 3 us each (1008, 16 best:
+// 105 and 43).
+struct BeamCounted {
+  int row, join;
+};
+BeamCounted be_counted(int K) {
+  const int few = std::min(23 * K, 256), many = (int)std::sqrt(256.0 * 23.0 * K);
+  return {std::min(std::max(few, many), BE_CAP),
+          std::min((int)std::sqrt(30720.0 * K), BE_JCAP)};
 }
 
 int be_workspace(pz_sampler* s) {
@@ -816,9 +874,9 @@ extern "C" int pz_beam_select(pz_sampler* s, const float* d_logits, long ld, int
   const int rc = be_workspace(s);
   if (rc != PZ_OK) return rc;
   const int64_t rows = (int64_t)n_groups * W;
-  constexpr int LONG = 256 * 32, SHORT = 256 * 8;
-  const bool few = rows * ((V + LONG - 1) / LONG) < 2 * (int64_t)s->n_cu;
-  const int S = few ? (V + SHORT - 1) / SHORT : (V + LONG - 1) / LONG;
+  const bool few = rows * ((V + BE_LONG - 1) / BE_LONG) < 2 * (int64_t)s->n_cu;
+  const int S = few ? (V + BE_SHORT - 1) / BE_SHORT : (V + BE_LONG - 1) / BE_LONG;
+  const BeamCounted counted = be_counted(K);
   const size_t per = (size_t)W * S * (sizeof(BeamStat) + (size_t)K * sizeof(uint64_t));
   int64_t step = (int64_t)(PZ_BEAM_WORKSPACE / per);
   const int64_t most = UINT32_MAX / 512 / ((int64_t)W * S);  // groups that a launch takes
@@ -835,6 +893,8 @@ extern "C" int pz_beam_select(pz_sampler* s, const float* d_logits, long ld, int
                         K,
                         1.0f / (float)(W * S),
                         1.0f / (float)S,
+                        counted.row,
+                        counted.join,
                         d_scores + g * W,
                         d_done ? d_done + g * W : nullptr,
                         pad_id,
