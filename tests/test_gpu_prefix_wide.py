@@ -171,3 +171,13 @@ def test_replayed(torch_cuda, sampler):
     c.lens, c.plens = d["lens"].cpu().numpy(), d["plens"].cpu().numpy()
     bs = [0, 3, 69, 70, 74, 75, 137, 139]
     some(c, bs).check(d["out"][bs], "the last")
+
+
+@pytest.mark.parametrize("kv,B,positions", [(1, 2, 300), (1, 2, 700), (512, 1, 300), (256, 1, 700)])
+def test_the_most_rows_of_a_sequence(torch_cuda, sampler, kv, B, positions):
+    """32768 of 64 elements, and no more: 512 heads of 64 nodes, over one key head to one
+    each."""
+    T, heads, D = 64, 512, 64
+    c = Shared(torch_cuda, "bf16", [positions], None, [40, 0][:B], T, heads, kv, D, 16,
+               seed=kv + positions).random_tree(3)
+    c.run(sampler, (kv, positions))
