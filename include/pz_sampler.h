@@ -527,12 +527,15 @@ typedef struct {
  * one softmax.  Arguments, results, rounding and refusals as pz_tree_attention (a
  * softmax weight is rounded against the largest score of the keys that its workgroup
  * reads); also, T * n_heads is at most 32768 (32513 with heads of 256).  All sequences'
- * rows of a key head meet the prefix's keys together, so that its bytes do not grow with
- * the sequences.
+ * rows of a key head meet the prefix's keys together, 16 to 256 rows at a time by how many
+ * a prefix has on average, so that its bytes grow little with the sequences.
  * Asynchronous on the sampler's stream, in pz_tree_attention's workspace, which the
  * first call of either allocates; after that call it can be captured into a HIP
  * graph.  Calls of both on one sampler, replays included, must be ordered.
- * With d_first n_prefixes is at most 4096. */
+ * With d_first n_prefixes is at most 4096, and the average is over all ranges, since only
+ * the device knows which are empty: a table with room for more than are in use costs time
+ * (256 sequences under one prefix of 4096 positions 49 us, 60 as one of 4 ranges whose
+ * others are empty, 110 as one of 150). */
 PZ_API int pz_prefix_attention(pz_sampler *s, const pz_kv_cache *cache,
                                const pz_kv_prefix *prefix, const void *d_kn, const void *d_vn,
                                long ld_n, int B, int T, const int32_t *d_n_nodes,
@@ -573,10 +576,11 @@ typedef struct {
  * and k may be parts of one row (of a fused projection).  d_q_out == d_q with equal
  * strides works in place, and d_k_out == d_k alike; outputs must not overlap the
  * inputs otherwise.  Without queries (n_heads = 0, d_q and d_q_out NULL) or without
- * keys alike.  Angles are meant to stay below 2^50 radians.  Pointers, strides and heads
- * that are multiples of 16 bytes are the quick case; at most 65536 heads of queries and of
- * keys, and n times both at most 2^26 - 1.  Asynchronous on the sampler's stream; uses no
- * workspace and can be captured into a HIP graph. */
+ * keys alike.  An angle is off by at most 3 2^-53 of itself (below 2^-24 up to 2^27
+ * radians, 2^-20 at 2^31); those of 2^50 radians and more are unspecified.  Pointers,
+ * strides and heads that are multiples of 16 bytes are the quick case; at most 65536
+ * heads of queries and of keys, and n times both at most 2^26 - 1.  Asynchronous on the
+ * sampler's stream; uses no workspace and can be captured into a HIP graph. */
 PZ_API int pz_qk_norm_rope(pz_sampler *s, const pz_qk_rope *rope, const void *d_q, long ld_q,
                            const void *d_k, long ld_k, void *d_q_out, long ld_q_out,
                            void *d_k_out, long ld_k_out, int n, const int32_t *d_pos);
@@ -628,7 +632,9 @@ PZ_API int pz_beam_select(pz_sampler *s, const float *d_logits, long ld, int n_g
  *     names any more is free again: new pages are the lowest free ones, given out in the
  *     order of beams and positions.  W * max_blocks pages always suffice; tables may also
  *     name pages outside the pool (a prompt's), which are shared and never given out (one
- *     that L ends in is the first child's to fill, so that no other group may read it).
+ *     that L ends in is the first child's to fill, so that no other group may read it,
+ *     nor another beam's table name it: beams share full pages only, as reorderings leave
+ *     them).
  *     Groups' pools must not have pages in common.
  *   d_missing [n_groups] or NULL: how many pages the pool lacked (those entries are
  *     -1, and what would have been copied is left out), 0 where all is well.

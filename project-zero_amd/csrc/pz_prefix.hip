@@ -16,6 +16,9 @@
 //   8 of up to 4096, 8 beams each (119 MB): 33 + 5.5, 3.6 TB/s in the first; twice the
 //     splits 4 us more, half of them 7
 //   1 of up to 32768, 256 sequences of up to 512 (104 GFLOP, 374 MB): 176 + 10
+// The weights' rounding to 16 bits for their product with the values takes results to 2.1e-3 to
+// 2.3e-3 of their norm from 64 bits in bf16 (1.65e-3 rounded once from 32 bits), to 2.8e-4 in
+// fp16 (2.1e-4).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

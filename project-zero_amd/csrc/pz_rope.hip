@@ -3,11 +3,11 @@
 //
 //   y = x w / sqrt(mean(x^2) + eps);  (a, b) -> (a cos - b sin, b cos + a sin) amplitude
 //
-// The angle pos * freq is wanted modulo a turn, to fp32's precision, for positions of
-// any size: in 64 bits, in quarter turns, t = pos * (freq 2 / pi), whose distance to
-// the nearest whole number (at most a half: at most pi / 4) is left for fp32, where
-// the series of sine and cosine stop after x^9 and x^10 (terms of 2e-9 and 1e-10 are
-// left out at pi / 4).
+// The angle pos * freq is wanted modulo a turn.  In 64 bits, in quarter turns, t = pos * (freq
+// 2 / pi) is off by at most 3 2^-53 of itself (below 2^-24 up to 2^27 radians); its distance to
+// the nearest whole number (at most a half: at most pi / 4), which is exact below 2^51 quarters,
+// is left for fp32, where the series of sine and cosine stop after x^9 and x^10 (terms of 2e-9
+// and 1e-10 are left out at pi / 4).
 //
 // k_qk_rope: a head is LG lanes, each of which owns two 16-byte vectors: of the same
 // place in the two halves (ROPE_HALVES; past the rotated part, the next two), or
